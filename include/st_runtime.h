@@ -261,6 +261,102 @@ int st_batch_device_run(st_batch* batch, const float* inputs, size_t count, doub
  * changes nothing. No counterpart in the reference, which has no batched streams. */
 int st_batch_set_eager(st_batch* batch, int32_t eager);
 
+/* ------------------------------------------------------------------------------------------
+ * Cache operators (extension; the reference's step has them fused, for one stream and a plain
+ * window, src/cuda/Primitives.cuh:148-219): what a model's attention does between its Q/K/V
+ * projection and its output projection, on the caller's device memory and stream.
+ *
+ * They check their arguments on the host before any device work, launch on `stream` (a
+ * hipStream_t of the current device; NULL is the default stream), and do not synchronize,
+ * allocate or copy, so they can be captured into a graph. All pointers inside the argument
+ * structs are device memory. Calls on one cache run in the order of their streams; calls whose
+ * work may overlap need caches, outputs and workspaces of their own. */
+
+/* Element types. INT4 is a cache's storage only. */
+enum { ST_TYPE_F32 = 0, ST_TYPE_F16 = 1, ST_TYPE_BF16 = 2, ST_TYPE_INT4 = 3 };
+
+/* A cache of keys and values with a sliding window and sinks (first positions that stay
+ * visible). For each stream and head it has sinks + ring rows (slots): position p lives in slot p
+ * where p < sinks, else in slot sinks + (p - sinks) mod ring. A query at position t sees the
+ * positions p <= t with p < sinks or p > t - window.
+ * Rows are head_dim elements (a multiple of 8, 8 to 256) of `dtype`. INT4 rows (head_dim a
+ * multiple of 32) are head_dim / 2 bytes of codes 0..15, in each little-endian 32-bit word of
+ * eight codes element 2j in bits 4j..4j+3 and element 2j + 1 in bits 16+4j..; and in key_params
+ * and value_params one FP16 pair (scale, minimum) for each 32 elements: a code stands for
+ * minimum + scale * code.
+ * Row (stream b, head h, slot s) is row b * stream_stride + h * head_stride + s * slot_stride of
+ * `keys` and `values` (16-byte aligned) and of the params (4-byte aligned); all three strides 0:
+ * contiguous [streams][kv_heads][slots].
+ * positions[b] (device memory) is the number of tokens that stream b had before the call: the
+ * position of its first new token. The calls read it and leave it; the caller adds the new tokens
+ * once every layer's calls are done. A negative position leaves the stream out of the call: its
+ * rows of the cache and of the outputs stay as they are. */
+typedef struct {
+  int32_t streams, kv_heads, head_dim;
+  int32_t window, sinks, ring;
+  int32_t dtype;
+  int64_t stream_stride, head_stride, slot_stride; /* in rows */
+  void* keys;
+  void* values;
+  void* key_params;   /* INT4 only */
+  void* value_params;
+  const int64_t* positions;
+} st_kv_cache;
+
+/* The rows of a call's new tokens: of stream b the rows offsets[b] .. offsets[b + 1] - 1 (device
+ * memory, streams + 1 entries, not decreasing), none or up to max_tokens; with offsets NULL the
+ * max_tokens rows from b * max_tokens on. Rows that belong to no stream stay as they are. A
+ * stream's rows past max_tokens, or past `tokens`, are left out. max_tokens may be at most
+ * ring - window + 1: then no token of a call overwrites a row that another one's query sees, and
+ * the results do not depend on how a prompt is cut into calls. tokens == 0 does nothing. */
+typedef struct {
+  int32_t tokens;     /* rows in all */
+  int32_t max_tokens; /* most rows of one stream */
+  const int32_t* offsets;
+} st_new_rows;
+
+/* Norm of each query and key head (x / sqrt(mean(x^2) + epsilon) * gain; none where the gain is
+ * NULL), rotation of its first rope_dims elements by the token's angles, and the append of keys and
+ * values to the cache, in one pass. Element (2i, 2i + 1) pairs, or (i, i + rope_dims / 2) with
+ * rope_halves, are rotated by position * inv_freq[i] radians, or by the rotation (cos, sin) at
+ * rope[(row * rope_dims / 2 + i) * 2]: one of the two must be given where rope_dims > 0.
+ * q, k, v and q_out hold [token][head][head_dim] of `dtype` with the given strides in elements
+ * (token, head; multiples of 16 bytes, the head's elements adjacent); q_out may be q. FP32 rows
+ * go with every cache type, FP16 and BF16 rows with a cache of their own type or INT4. Values are
+ * rounded once, to the nearest of the output's or cache's type; an INT4 group with a value that is
+ * not finite reads back as NaN, and values beyond FP16's range do not survive in one. */
+typedef struct {
+  int32_t dtype, q_heads;
+  const void *q, *k, *v;
+  void* q_out;
+  int64_t q_strides[2], k_strides[2], v_strides[2], out_strides[2];
+  const float *q_gain, *k_gain; /* [head_dim] or NULL */
+  float epsilon;
+  int32_t rope_dims, rope_halves;
+  const double* inv_freq; /* [rope_dims / 2] */
+  const float* rope;      /* [tokens][rope_dims / 2][2] */
+} st_append_args;
+int st_qk_norm_rope_append(const st_kv_cache* cache, const st_new_rows* rows, const st_append_args* args,
+                           void* stream);
+
+/* Attention of the new tokens' queries over the cache, which holds their keys and values already:
+ * softmax(scale * q . K) V over the positions that a query sees. q_heads is a multiple of
+ * kv_heads, and query head h reads cache head h / (q_heads / kv_heads). Strides and types as above.
+ * The workspace holds st_window_attention_workspace's bytes (which depend on the structs' numbers
+ * alone; 0: none needed) and is 16-byte aligned; its contents matter during the call only. */
+typedef struct {
+  int32_t dtype, q_heads;
+  const void* q;
+  void* out;
+  int64_t q_strides[2], out_strides[2];
+  float scale;
+  void* workspace;
+  size_t workspace_bytes;
+} st_attention_args;
+int st_window_attention_workspace(const st_kv_cache* cache, const st_new_rows* rows, int32_t q_heads, int32_t dtype,
+                                  size_t* bytes);
+int st_window_attention(const st_kv_cache* cache, const st_new_rows* rows, const st_attention_args* args, void* stream);
+
 /* Message of the last failed call on this thread ("" if none). */
 const char* st_last_error(void);
 

@@ -1,0 +1,631 @@
+// Attention over a sliding-window cache: softmax(scale * q . K) V over the positions that a query sees
+// (cache_device.hpp). Queries of the same stream and key/value head share the cache rows: a row of the
+// matrix products is a (token, query head) pair, head fastest.
+//
+// One pass over the keys with the softmax's running maximum m and sum l per row, in 32 bits, in the base
+// of two. For a tile of keys S^T = K Q^T and O^T += V^T P^T, both on MFMA 16x16: with the rows of the
+// products on the lanes (lane % 16), the maximum, the sum and the rescaling are per lane, and the four keys
+// (4 (lane / 16) + i) that a lane holds of each 16 x 16 block of S^T are, rounded, the operand that P^T
+// wants. The order of the keys within a product's depth does not matter as long as both operands agree.
+#pragma once
+
+#include "cache_device.hpp"
+
+namespace stamd {
+
+struct AttentionView {
+  const char* q;
+  char* out;
+  int64_t q_token, q_head, out_token, out_head;  // strides in bytes
+  float scale;       // times log2(e)
+  int group;         // query heads per key/value head
+  int rows;          // most rows of a (stream, key/value head): max_tokens * group
+  int splits;        // workgroups along the keys
+  float2* part_ml;   // splits > 1: partial (m, l) [stream][kv head][row][split]
+  float* part_o;     // and output [stream][kv head][row][split][dim]
+  int out_layout;    // 0: strides above; 1, 2: the projections' operand layouts (act_index), out_ld columns
+  int out_ld;
+};
+
+// The keys that some query of the tokens ta .. tb (positions) sees, as a list: first the sinks, then the
+// ring's positions lo .. tb. j is an index into the list.
+struct KeyList {
+  int sinks, total;     // entries
+  int offset, ring, slots_sinks;  // ring slot of the first ring entry
+  int64_t lo;
+  __device__ __forceinline__ void init(const CacheView& c, int64_t ta, int64_t tb) {
+    sinks = (int)min((int64_t)c.sinks, tb + 1);
+    lo = max((int64_t)c.sinks, ta - c.window + 1);
+    const int64_t ringed = tb - lo + 1;
+    total = sinks + (ringed > 0 ? (int)ringed : 0);
+    offset = ringed > 0 ? ring_offset(c, lo) : 0;
+    ring = c.ring;
+    slots_sinks = c.sinks;
+  }
+  __device__ __forceinline__ int slot(int j) const {
+    const int o = offset + j - sinks;
+    return j < sinks ? j : slots_sinks + (o >= ring ? o - ring : o);
+  }
+};
+// What one query at position t sees of a list: sinks up to t, ring entries in (newest - window, newest].
+struct Seen {
+  int t, newest;
+  __device__ __forceinline__ void init(const KeyList& k, int64_t position) {
+    t = (int)min(position, (int64_t)1 << 30);
+    newest = (int)max(position - k.lo, (int64_t)-1);
+  }
+  __device__ __forceinline__ bool operator()(const KeyList& k, int window, int j) const {
+    const int e = j - k.sinks;
+    return j < k.total && (e < 0 ? j <= t : e <= newest && e > newest - window);
+  }
+};
+
+// A tile of K and V rows in LDS, the elements that the MFMAs take: FP32, or 16 bits. Rows are D elements
+// (the head dimension padded with zeros to 64, 128 or 256) in 16-byte chunks; chunk c of row r is stored
+// at c ^ swizzle(r), which spreads over the banks what 16 lanes read at once: one chunk of 16 rows (K),
+// 32 bytes of 16 rows (V, transposed 16-bit reads), 64 bytes of four rows (V, FP32).
+template <int M, int D>
+struct TileLayout {
+  static constexpr int kElem = M == kTF32 ? 4 : 2;
+  static constexpr int kRow = D * kElem, kChunks = kRow / 16;
+  __device__ static __forceinline__ int key_chunk(int r, int c) { return c ^ (kChunks == 8 ? (r >> 1) & 7 : r & 15); }
+  __device__ static __forceinline__ int value_chunk(int r, int c) {
+    if constexpr (M == kTF32) return c ^ (((r >> 2) & 3) << 2);
+    else if constexpr (kChunks == 8) return c ^ (((r >> 1) & 3) << 1);
+    else return c ^ ((r & 7) << 1);
+  }
+};
+
+// How rows of cache type C come in 16-byte loads: E elements each, L lanes per row.
+template <int C, int D>
+struct RowLoad {
+  static constexpr int E = C == kTF32 ? 4 : C == kTInt4 ? 32 : 8;
+  static constexpr int L = D / E;
+};
+
+// The 32 codes of a 4-bit load and their (scale, minimum) as 16-bit or FP32 values. FP16: code + 1024 (or
+// + 64 for the codes in bits 4 and 12 of a half) is made by an OR, the constant subtracted exactly, and
+// minimum + scale * code is rounded once, to FP16 (2^-12 of the value, for 16-bit queries only).
+__device__ __forceinline__ word4_t dequant8_f16(unsigned w, half2_t s, half2_t z) {
+  const half2_t big = {(_Float16)1024.f, (_Float16)1024.f}, mid = {(_Float16)64.f, (_Float16)64.f};
+  auto a = [&](unsigned x) {
+    return __builtin_bit_cast(unsigned, (__builtin_bit_cast(half2_t, (x & 0x000f000fu) | 0x64006400u) - big) * s + z);
+  };
+  auto b = [&](unsigned x) {
+    return __builtin_bit_cast(unsigned, (__builtin_bit_cast(half2_t, (x & 0x00f000f0u) | 0x54005400u) - mid) * s + z);
+  };
+  return word4_t{a(w), b(w), a(w >> 8), b(w >> 8)};
+}
+__device__ __forceinline__ void dequant8_f32(unsigned w, float s, float z, float4_t (&out)[2]) {
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    out[j >> 1][(j & 1) * 2] = z + s * (float)((w >> (4 * j)) & 15u);
+    out[j >> 1][(j & 1) * 2 + 1] = z + s * (float)((w >> (16 + 4 * j)) & 15u);
+  }
+}
+
+// One 16-byte load of row r, lane position p of the row's L, as the chunks of the LDS tile: calls
+// put(chunk, value) for each. `keep`: whether the lane's elements are inside the head.
+template <int C, int M, typename Put>
+__device__ __forceinline__ void expand(word4_t w, unsigned params, int p, bool keep, Put&& put) {
+  if (!keep) {
+    w = word4_t{0, 0, 0, 0};
+    params = 0;
+  }
+  if constexpr (C == M) {
+    put(p, w);
+  } else if constexpr (C == kTInt4) {
+    const half2_t sz = __builtin_bit_cast(half2_t, params);
+    if constexpr (M == kTF32) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        float4_t f[2];
+        dequant8_f32(w[i], (float)sz[0], (float)sz[1], f);
+        put(p * 8 + 2 * i, __builtin_bit_cast(word4_t, f[0]));
+        put(p * 8 + 2 * i + 1, __builtin_bit_cast(word4_t, f[1]));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++) put(p * 4 + i, dequant8_f16(w[i], half2_t{sz[0], sz[0]}, half2_t{sz[1], sz[1]}));
+    }
+  } else {
+    static_assert(M == kTF32);
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      put(p * 2 + i, __builtin_bit_cast(word4_t, float4_t{low16<C>(w[2 * i]), high16<C>(w[2 * i]), low16<C>(w[2 * i + 1]),
+                                                          high16<C>(w[2 * i + 1])}));
+    }
+  }
+}
+// Whether a chunk of the tile holds a value that is not finite.
+template <int M>
+__device__ __forceinline__ bool not_finite(word4_t w) {
+  constexpr unsigned e = M == kTF32 ? 0x7f800000u : M == kTF16 ? 0x7c00u : 0x7f80u;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if constexpr (M == kTF32) bad |= (w[i] & e) == e;
+    else bad |= (w[i] & e) == e || ((w[i] >> 16) & e) == e;
+  }
+  return bad;
+}
+
+template <int M>
+struct Mfma {
+  // Two 16-byte fragments (4 FP32 or 8 16-bit elements of depth per lane): D += A B^T.
+  __device__ static __forceinline__ float4_t mul(word4_t a, word4_t b, float4_t d) {
+    if constexpr (M == kTF16) {
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), d, 0, 0, 0);
+    } else if constexpr (M == kTB16) {
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bhalf8_t, a), __builtin_bit_cast(bhalf8_t, b), d, 0, 0,
+                                                     0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++) d = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_to_float(a[i]), bits_to_float(b[i]), d, 0, 0, 0);
+      return d;
+    }
+  }
+};
+
+typedef __attribute__((address_space(3))) char lds_char;
+template <typename T>
+__device__ __forceinline__ T lds_load(const char* p) {
+  return *(const __attribute__((address_space(3))) T*)p;
+}
+template <typename T>
+__device__ __forceinline__ void lds_put(char* p, T v) {
+  *(__attribute__((address_space(3))) T*)p = v;
+}
+// Four 16-bit elements of one column and four consecutive rows: 16 lanes read a 4 x 16 block, lane i at
+// row i / 4, elements 4 (i % 4) ..; lane i receives column i.
+__device__ __forceinline__ word2_t lds_column4(const char* p) {
+  return __builtin_bit_cast(word2_t,
+                            __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)p));
+}
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// The type that the MFMAs take: FP32 for FP32 queries (every cache type widens to it exactly), else the
+// queries' own; 4-bit rows become FP16 for bfloat16 queries too, whose eight significant bits FP16 holds
+// once the row is scaled by a power of two.
+template <int A, int C>
+constexpr int mfma_type() {
+  return A == kTF32 ? kTF32 : C == kTInt4 ? kTF16 : A;
+}
+
+// The queries' fragments of one block of 16 rows, lane % 16 the row: 16 bytes per step of kStep dims.
+// factor: what a logit in the base of two is of the products.
+template <int A, int M, int D>
+struct QueryBlock {
+  static constexpr int kStep = M == kTF32 ? 16 : 32, kSteps = D / kStep;
+  word4_t f[kSteps];
+  float factor;
+  __device__ __forceinline__ void load(const char* row, int dim, float scale, int g, bool valid) {
+    factor = scale;
+    constexpr int per = kStep / 4;  // dims of a lane per step
+    if constexpr (A == M) {
+#pragma unroll
+      for (int s = 0; s < kSteps; s++) {
+        const int d = s * kStep + g * per;
+        const word4_t w = load_global<word4_t>(row + (d < dim ? d : 0) * (A == kTF32 ? 4 : 2));
+        f[s] = valid && d < dim ? w : word4_t{0, 0, 0, 0};
+      }
+    } else {  // bfloat16 to FP16
+      float x[kSteps][8], top = 0.f;
+#pragma unroll
+      for (int s = 0; s < kSteps; s++) {
+        const int d = s * kStep + g * per;
+        const bool in = valid && d < dim;
+        const word4_t w = load_global<word4_t>(row + (d < dim ? d : 0) * 2);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          x[s][2 * i] = in ? low16<kTB16>(w[i]) : 0.f;
+          x[s][2 * i + 1] = in ? high16<kTB16>(w[i]) : 0.f;
+          top = fmaxf(top, fmaxf(fabsf(x[s][2 * i]), fabsf(x[s][2 * i + 1])));
+        }
+      }
+      top = pair32_max(pair16_max(top));
+      // 2^e with e the exponent of the row's largest value; rows of zeros, and rows that are not finite,
+      // stay as they are.
+      const unsigned e = (float_to_bits(top) >> 23) & 255u;
+      const bool plain = e == 0 || e >= 254;
+      const float down = plain ? 1.f : bits_to_float((254u - e) << 23);
+      factor = plain ? scale : scale * bits_to_float(e << 23);
+#pragma unroll
+      for (int s = 0; s < kSteps; s++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) f[s][i] = pack_f16(x[s][2 * i] * down, x[s][2 * i + 1] * down);
+    }
+  }
+};
+
+// Products of one tile with a block of 16 rows, for a wave. kt and vt: the tile's K and V in LDS.
+template <int M, int D, int KT>
+struct TileMath {
+  using T = TileLayout<M, D>;
+  static constexpr int kBlocks = KT / 16;
+  // S^T of one block of 16 keys for each of MB blocks of rows.
+  template <int MB, typename Q>
+  __device__ static __forceinline__ void logits(const char* kt, int kb, const Q (&q)[MB], float4_t (&s)[MB], int lane) {
+    const int r = kb * 16 + (lane & 15), g = lane >> 4;
+#pragma unroll
+    for (int m = 0; m < MB; m++) s[m] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int step = 0; step < Q::kSteps; step++) {
+      const word4_t k = lds_load<word4_t>(kt + r * T::kRow + T::key_chunk(r, step * 4 + g) * 16);
+#pragma unroll
+      for (int m = 0; m < MB; m++) s[m] = Mfma<M>::mul(k, q[m].f[step], s[m]);
+    }
+  }
+  // The V operand of 16 dims (block db) and one depth of P: 32 keys (blocks 2 d, 2 d + 1), FP32 16 keys.
+  __device__ static __forceinline__ word4_t values(const char* vt, int depth, int db, int lane) {
+    const int i = lane & 15, g = lane >> 4;
+    if constexpr (M == kTF32) {
+      word4_t v;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const int r = depth * 16 + g * 4 + e;
+        v[e] = lds_load<unsigned>(vt + r * T::kRow + T::value_chunk(r, db * 4 + (i >> 2)) * 16 + (i & 3) * 4);
+      }
+      return v;
+    } else {
+      word2_t h[2];
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const int r = depth * 32 + e * 16 + g * 4 + (i >> 2);
+        h[e] = lds_column4(vt + r * T::kRow + T::value_chunk(r, db * 2 + ((i & 3) >> 1)) * 16 + (i & 1) * 8);
+      }
+      return word4_t{h[0][0], h[0][1], h[1][0], h[1][1]};
+    }
+  }
+  static constexpr int kDepth = M == kTF32 ? 16 : 32, kDepths = KT / kDepth;
+  // The operand P^T of one depth from the blocks' weights p[block][i].
+  __device__ static __forceinline__ word4_t weights(const float4_t (&p)[kBlocks], int depth) {
+    if constexpr (M == kTF32) {
+      return __builtin_bit_cast(word4_t, p[depth]);
+    } else {
+      const float4_t a = p[2 * depth], b = p[2 * depth + 1];
+      return word4_t{pack16<M>(a[0], a[1]), pack16<M>(a[2], a[3]), pack16<M>(b[0], b[1]), pack16<M>(b[2], b[3])};
+    }
+  }
+  // Tiles that are not seen whole and hold values of V that are not finite: adds such values to the
+  // outputs of the rows that see them, then makes them zeros in LDS, so that the products add nothing.
+  template <int MB, typename Sees>
+  __device__ static __forceinline__ void settle(char* vt, float4_t (&o)[MB][D / 16], int lane, Sees&& sees) {
+    const int g = lane >> 4;
+#pragma unroll 1
+    for (int r = 0; r < KT; r++) {
+      bool seen[MB];
+#pragma unroll
+      for (int u = 0; u < MB; u++) seen[u] = sees(u, r);
+#pragma unroll
+      for (int db = 0; db < D / 16; db++) {
+        float v[4];
+        if constexpr (M == kTF32) {
+          const float4_t x = lds_load<float4_t>(vt + r * T::kRow + T::value_chunk(r, db * 4 + g) * 16);
+#pragma unroll
+          for (int i = 0; i < 4; i++) v[i] = x[i];
+        } else {
+          const word2_t x = lds_load<word2_t>(vt + r * T::kRow + T::value_chunk(r, db * 2 + (g >> 1)) * 16 + (g & 1) * 8);
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            v[2 * i] = low16<M>(x[i]);
+            v[2 * i + 1] = high16<M>(x[i]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float bad = v[i] - v[i] == 0.f ? 0.f : v[i];
+#pragma unroll
+          for (int u = 0; u < MB; u++) o[u][db][i] += seen[u] ? bad : 0.f;
+        }
+      }
+    }
+    wave_sync();
+#pragma unroll 1
+    for (int at = lane * 16; at < KT * T::kRow; at += 64 * 16) {
+      word4_t w = lds_load<word4_t>(vt + at);
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        if constexpr (M == kTF32) {
+          w[i] = (w[i] & 0x7f800000u) == 0x7f800000u ? 0u : w[i];
+        } else {
+          constexpr unsigned e = M == kTF16 ? 0x7c00u : 0x7f80u;
+          w[i] = ((w[i] & e) == e ? 0u : w[i] & 0xffffu) | (((w[i] >> 16) & e) == e ? 0u : w[i] & 0xffff0000u);
+        }
+      }
+      lds_put(vt + at, w);
+    }
+    wave_sync();
+  }
+};
+
+constexpr int kAttentionThreads = 256;  // cache_attention's workgroup: four waves
+
+// Keys of a wave's tile: 16 KB of K and V, or what one MFMA depth needs.
+template <int M, int D>
+constexpr int wave_tile() {
+  return M == kTF32 ? (D == 64 ? 32 : 16) : (D == 64 ? 64 : 32);
+}
+
+// The address of a pair of 16-byte (four FP32 or eight 16-bit) elements of the output row of (token row,
+// head h), elements d ..: four consecutive FP32 elements are consecutive in every layout.
+template <int A>
+__device__ __forceinline__ void store_out(const AttentionView& a, int row, int h, int dim, int d, const float (&x)[4]) {
+  if (A == kTF32 && a.out_layout) {
+    const int n = h * dim + d;
+    const size_t at = a.out_layout == 1 ? ((((size_t)(row >> 4) * (a.out_ld >> 4) + (n >> 4)) * 64 + (row & 15) + 16 * ((n & 15) >> 2)) * 4)
+                                        : (((((size_t)(row >> 4) * (a.out_ld >> 5) + (n >> 5)) * 2 + ((n >> 2) & 1)) * 64 + (row & 15) +
+                                            16 * ((n & 31) >> 3)) * 4);
+    store_global(a.out + at * 4, float4_t{x[0], x[1], x[2], x[3]});
+    return;
+  }
+  char* p = a.out + row * a.out_token + h * a.out_head + (int64_t)d * (A == kTF32 ? 4 : 2);
+  if constexpr (A == kTF32) store_global(p, float4_t{x[0], x[1], x[2], x[3]});
+  else store_global(p, word2_t{pack16<A>(x[0], x[1]), pack16<A>(x[2], x[3])});
+}
+
+// Few rows over many keys (decoding, short pieces): bound by reading the cache once. Workgroup (split,
+// kv head, row tile; stream): MB blocks of 16 rows. Its four waves take the keys' tiles in turn, each
+// with LDS of its own and no barrier in the loop; the next tile is in flight in registers while one is
+// computed. At the end the waves' (m, l, O) are merged through LDS. With splits > 1 the workgroup's own
+// are written instead, and cache_combine merges them.
+//
+// A masked key's weight is an exact zero, but zero times a value that is not finite is NaN: tiles that are
+// not seen whole look for such values as they are staged, and where there is one they are added apart, for
+// the rows that see them (TileMath::settle).
+template <int A, int C, int D, int MB>
+__global__ __launch_bounds__(kAttentionThreads, D == 256 ? 1 : 2) void cache_attention(CacheView c, RowsView r,
+                                                                                     AttentionView a) {
+  constexpr int M = mfma_type<A, C>();
+  constexpr int KT = wave_tile<M, D>();
+  using T = TileLayout<M, D>;
+  using R = RowLoad<C, D>;
+  using X = TileMath<M, D, KT>;
+  constexpr int kWaves = kAttentionThreads / 64;
+  constexpr int kPerLoad = 64 / R::L;                                // rows of one load of the wave
+  constexpr int kLoads = (KT + kPerLoad - 1) / kPerLoad;
+  static_assert(KT % kPerLoad == 0);
+  constexpr int kTile = KT * T::kRow;
+  constexpr int kMerge = MB * 16 * (D + 4) * 4;                      // a wave's O in the merge
+  constexpr int kWaveLds = 2 * kTile > kMerge ? 2 * kTile : kMerge;
+  __shared__ __attribute__((aligned(16))) char lds[kWaves * kWaveLds];
+  __shared__ float ml[kWaves][2][MB * 16];
+
+  const int split = blockIdx.x % a.splits, head = blockIdx.x / a.splits % c.kv_heads;
+  const int tile_of_rows = blockIdx.x / a.splits / c.kv_heads, b = blockIdx.y;
+  const int64_t start = c.positions[b];
+  int first, n;
+  stream_rows(r, b, first, n);
+  const int row0 = tile_of_rows * MB * 16, rows = n * a.group;
+  if (start < 0 || row0 >= rows) return;
+  const int last_row = min(row0 + MB * 16, rows) - 1;
+  const int64_t ta = start + row0 / a.group, tb = start + last_row / a.group;
+  KeyList keys;
+  keys.init(c, ta, tb);
+
+  const int wave = wave_id(), lane = lane_id(), g = lane >> 4;
+  char* kt = lds + wave * kWaveLds;
+  char* vt = kt + kTile;
+
+  // Loads of the tile that starts at list entry j0; entries past the end repeat the last.
+  const int p = lane % R::L, sub = lane / R::L;
+  const bool keep = p * R::E < c.dim;
+  const int64_t base_row = b * c.stream_stride + head * c.head_stride;
+  const char* kbase = c.keys + base_row * c.row_bytes + (keep ? p * 16 : 0);
+  const char* vbase = c.values + base_row * c.row_bytes + (keep ? p * 16 : 0);
+  const int pairs = C == kTInt4 ? c.dim / kQuantGroup : 0;
+  const uint32_t* kpbase = C == kTInt4 ? c.key_params + base_row * pairs + (keep ? p : 0) : nullptr;
+  const uint32_t* vpbase = C == kTInt4 ? c.value_params + base_row * pairs + (keep ? p : 0) : nullptr;
+  const uint32_t slot_bytes = c.slot_stride * c.row_bytes;
+  word4_t kw[kLoads], vw[kLoads];
+  unsigned kp[kLoads], vp[kLoads];
+  auto load = [&](int j0) {
+    int slot[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; i++) {
+      slot[i] = keys.slot(min(j0 + i * kPerLoad + sub, keys.total - 1));
+      kw[i] = load_global<word4_t>(kbase + (uint64_t)slot[i] * slot_bytes);
+    }
+#pragma unroll
+    for (int i = 0; i < kLoads; i++) vw[i] = load_global<word4_t>(vbase + (uint64_t)slot[i] * slot_bytes);
+    if constexpr (C == kTInt4) {
+#pragma unroll
+      for (int i = 0; i < kLoads; i++) {
+        const uint64_t at = (uint64_t)slot[i] * c.slot_stride * pairs;
+        kp[i] = load_global<unsigned>(kpbase + at);
+        vp[i] = load_global<unsigned>(vpbase + at);
+      }
+    }
+  };
+
+  const int tiles = (keys.total + KT - 1) / KT, per = (tiles + a.splits - 1) / a.splits;
+  const int t1 = min((split + 1) * per, tiles);
+  int tile = split * per + wave;
+  if (tile < t1) load(tile * KT);
+
+  QueryBlock<A, M, D> q[MB];
+  Seen seen[MB];
+  float m[MB], l[MB];
+  float4_t o[MB][D / 16];
+#pragma unroll
+  for (int u = 0; u < MB; u++) {
+    const int row = min(row0 + u * 16 + (lane & 15), last_row);
+    const int token = row / a.group, h = head * a.group + row - token * a.group;
+    q[u].load(a.q + (first + token) * a.q_token + h * a.q_head, c.dim, a.scale, g, row0 + u * 16 + (lane & 15) <= last_row);
+    seen[u].init(keys, start + token);
+    m[u] = -INFINITY;
+    l[u] = 0.f;
+#pragma unroll
+    for (int d = 0; d < D / 16; d++) o[u][d] = float4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  // List entries that every row sees: from whole_from on, up to whole_to (ring entries).
+  const int whole_from = keys.sinks + max((int)(tb - keys.lo) - c.window + 1, 0);
+  const int whole_to = keys.sinks + max((int)max(ta - keys.lo, (int64_t)-1) + 1, 0);
+  const int whole_sinks = (int)min((int64_t)keys.sinks, ta + 1);
+
+  for (; tile < t1; tile += kWaves) {
+    const int j0 = tile * KT;
+    // Whole: every row sees the tile's every entry.
+    const bool whole = (j0 >= whole_from && j0 + KT <= whole_to) || j0 + KT <= whole_sinks ||
+                       (whole_sinks == keys.sinks && whole_from == keys.sinks && j0 + KT <= whole_to);
+    bool odd = false;  // a value that is not finite in a tile that is not whole
+    wave_sync();
+#pragma unroll
+    for (int i = 0; i < kLoads; i++) {
+      const int row = i * kPerLoad + sub;
+      expand<C, M>(kw[i], kp[i], p, keep, [&](int ch, word4_t w) { lds_put(kt + row * T::kRow + T::key_chunk(row, ch) * 16, w); });
+      expand<C, M>(vw[i], vp[i], p, keep, [&](int ch, word4_t w) {
+        lds_put(vt + row * T::kRow + T::value_chunk(row, ch) * 16, w);
+        if (!whole) odd |= not_finite<M>(w);
+      });
+    }
+    odd = __ballot(odd) != 0;
+    if (tile + kWaves < t1) load((tile + kWaves) * KT);
+    wave_sync();
+
+    float4_t s[X::kBlocks][MB];
+#pragma unroll
+    for (int kb = 0; kb < X::kBlocks; kb++) X::logits(kt, kb, q, s[kb], lane);
+    float4_t pw[MB][X::kBlocks];
+#pragma unroll
+    for (int u = 0; u < MB; u++) {
+      float top = m[u];
+#pragma unroll
+      for (int kb = 0; kb < X::kBlocks; kb++) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          float x = s[kb][u][i] * q[u].factor;
+          if (!whole && !seen[u](keys, c.window, j0 + kb * 16 + g * 4 + i)) x = -INFINITY;
+          pw[u][kb][i] = x;
+          top = fmaxf(top, x);
+        }
+      }
+      top = pair32_max(pair16_max(top));
+      const float safe = top == -INFINITY ? 0.f : top;
+      if (__ballot(top != m[u])) {  // rows whose maximum stays have alpha 1
+        const float alpha = __builtin_amdgcn_exp2f(m[u] - safe);
+        l[u] *= alpha;
+#pragma unroll
+        for (int d = 0; d < D / 16; d++) o[u][d] *= alpha;
+        m[u] = top;
+      }
+#pragma unroll
+      for (int kb = 0; kb < X::kBlocks; kb++) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          pw[u][kb][i] = __builtin_amdgcn_exp2f(pw[u][kb][i] - safe);
+          l[u] += pw[u][kb][i];
+        }
+      }
+    }
+    if (odd) X::settle(vt, o, lane, [&](int u, int e) { return seen[u](keys, c.window, j0 + e); });
+#pragma unroll
+    for (int depth = 0; depth < X::kDepths; depth++) {
+      word4_t w[MB];
+#pragma unroll
+      for (int u = 0; u < MB; u++) w[u] = X::weights(pw[u], depth);
+#pragma unroll
+      for (int d = 0; d < D / 16; d++) {
+        const word4_t v = X::values(vt, depth, d, lane);
+#pragma unroll
+        for (int u = 0; u < MB; u++) o[u][d] = Mfma<M>::mul(v, w[u], o[u][d]);
+      }
+    }
+  }
+
+  // Merge of the four waves.
+#pragma unroll
+  for (int u = 0; u < MB; u++) {
+    l[u] = pair32_add(pair16_add(l[u]));
+    if (g == 0) {
+      ml[wave][0][u * 16 + (lane & 15)] = m[u];
+      ml[wave][1][u * 16 + (lane & 15)] = l[u];
+    }
+  }
+  __syncthreads();
+  float* merge = reinterpret_cast<float*>(lds);
+#pragma unroll
+  for (int u = 0; u < MB; u++) {
+    const int row = u * 16 + (lane & 15);
+    float top = ml[0][0][row];
+#pragma unroll
+    for (int w = 1; w < kWaves; w++) top = fmaxf(top, ml[w][0][row]);
+    const float f = m[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[u] - top);
+#pragma unroll
+    for (int d = 0; d < D / 16; d++) {
+      const float4_t x = o[u][d] * f;
+      *(float4_t*)(merge + (wave * MB * 16 + row) * (D + 4) + d * 16 + g * 4) = x;
+    }
+  }
+  __syncthreads();
+  const int quads = c.dim / 4;
+  for (int i = threadIdx.x; i < (last_row - row0 + 1) * quads; i += kAttentionThreads) {
+    const int row = i / quads, d = (i - row * quads) * 4;
+    float top = ml[0][0][row], sum = 0.f;
+#pragma unroll
+    for (int w = 1; w < kWaves; w++) top = fmaxf(top, ml[w][0][row]);
+    float4_t x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) {
+      const float mw = ml[w][0][row];
+      sum += mw == -INFINITY ? ml[w][1][row] : ml[w][1][row] * __builtin_amdgcn_exp2f(mw - top);
+      x += *(const float4_t*)(merge + (w * MB * 16 + row) * (D + 4) + d);
+    }
+    if (a.splits > 1) {
+      const size_t at = (((size_t)b * c.kv_heads + head) * a.rows + row0 + row) * a.splits + split;
+      if (d == 0) a.part_ml[at] = make_float2(top, sum);
+      store_global(a.part_o + at * c.dim + d, x);
+    } else {
+      const int token = (row0 + row) / a.group, h = head * a.group + row0 + row - token * a.group;
+      const float inv = 1.f / sum;
+      const float y[4] = {x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
+      store_out<A>(a, first + token, h, c.dim, d, y);
+    }
+  }
+}
+
+constexpr int kMaxSplits = 64;
+
+// The splits of each row merged: workgroup (row, kv head, stream), 64 lanes of four elements times four
+// shares of the splits, joined in a fixed order.
+template <int A>
+__global__ __launch_bounds__(256) void cache_combine(CacheView c, RowsView r, AttentionView a) {
+  __shared__ float weight[kMaxSplits];
+  __shared__ float4_t part[4][64];
+  const int row = blockIdx.x, head = blockIdx.y, b = blockIdx.z;
+  int first, n;
+  stream_rows(r, b, first, n);
+  if (c.positions[b] < 0 || row >= n * a.group) return;
+  const size_t at = (((size_t)b * c.kv_heads + head) * a.rows + row) * a.splits;
+  const int lane = lane_id(), wave = wave_id();
+  const float2 ml = lane < a.splits ? a.part_ml[at + lane] : make_float2(-INFINITY, 0.f);
+  const float top = wave_top(ml.x);
+  const float w = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - top);
+  const float sum = wave_total(ml.x == -INFINITY ? ml.y : ml.y * w);
+  if (wave == 0) weight[lane] = w;
+  __syncthreads();
+  const int d = lane * 4;
+  float4_t x = {0.f, 0.f, 0.f, 0.f};
+  if (d < c.dim) {
+#pragma unroll 4
+    for (int s = wave; s < a.splits; s += 4) {
+      const float4_t v = load_global<float4_t>(a.part_o + (at + s) * c.dim + d);
+      if (weight[s] != 0.f) x += v * weight[s];
+    }
+  }
+  part[wave][lane] = x;
+  __syncthreads();
+  if (wave == 0 && d < c.dim) {
+    x = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+    const float inv = 1.f / sum;
+    const float y[4] = {x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
+    const int token = row / a.group, h = head * a.group + row - token * a.group;
+    store_out<A>(a, first + token, h, c.dim, d, y);
+  }
+}
+
+}  // namespace stamd

@@ -30,6 +30,28 @@ struct Error : std::runtime_error {
       throw Error(ST_ERR_DEVICE, std::string(#expr) + ": " + hipGetErrorString(_e));       \
   } while (0)
 
+// The message of the calling thread's last failed call (defined in runtime.hip), and the body of a C entry
+// point: no exception leaves it.
+extern thread_local std::string g_last_error;
+
+template <class F>
+int guarded(F&& f) {
+  try {
+    f();
+    g_last_error.clear();
+    return ST_OK;
+  } catch (const Error& e) {
+    g_last_error = e.what();
+    return e.code;
+  } catch (const std::exception& e) {
+    g_last_error = e.what();
+    return ST_ERR_DEVICE;
+  } catch (...) {
+    g_last_error = "unknown error";
+    return ST_ERR_DEVICE;
+  }
+}
+
 // Events that only time device work between launches. Recorded without the system-scope
 // fence (an L2 writeback and invalidation before every record), so consecutive steps run as they
 // would untimed; the host reads results only after synchronizing the stream, which releases at

@@ -32,7 +32,7 @@
 
 namespace stamd {
 
-static thread_local std::string g_last_error;
+thread_local std::string g_last_error;
 
 static std::string json_escape(const std::string& s) {
   std::string o;
@@ -1468,23 +1468,7 @@ struct st_runtime {
   std::unique_ptr<stamd::Runtime> impl;
 };
 
-template <class F>
-static int guarded(F&& f) {
-  try {
-    f();
-    stamd::g_last_error.clear();
-    return ST_OK;
-  } catch (const stamd::Error& e) {
-    stamd::g_last_error = e.what();
-    return e.code;
-  } catch (const std::exception& e) {
-    stamd::g_last_error = e.what();
-    return ST_ERR_DEVICE;
-  } catch (...) {
-    stamd::g_last_error = "unknown error";
-    return ST_ERR_DEVICE;
-  }
-}
+using stamd::guarded;
 
 namespace stamd {
 

@@ -8,7 +8,7 @@ import sys
 from pathlib import Path
 
 PACKAGE_DIR = Path(__file__).resolve().parent.parent
-SOURCES = [PACKAGE_DIR / 'csrc' / 'runtime.hip', PACKAGE_DIR / 'csrc' / 'batch.hip']
+SOURCES = [PACKAGE_DIR / 'csrc' / name for name in ('runtime.hip', 'batch.hip', 'cache_ops.hip')]
 DEPENDS = SOURCES + list((PACKAGE_DIR / 'csrc').glob('*.hpp')) + [PACKAGE_DIR.parent / 'include' / 'st_runtime.h']
 OUTPUT = PACKAGE_DIR / 'lib' / 'libstamd.so'
 

@@ -121,7 +121,11 @@ def library(path: os.PathLike | None = None) -> ctypes.CDLL:
     lib.st_batch_snapshot.argtypes = [P, ctypes.c_int32, ctypes.POINTER(ctypes.c_uint64), F, F, F]
     lib.st_batch_device_run.argtypes = [P, F, ctypes.c_size_t, D, D]
     lib.st_batch_set_eager.argtypes = [P, ctypes.c_int32]
-    for name in ('st_batch_create', 'st_batch_create_resident', 'st_batch_step', 'st_batch_reset', 'st_batch_snapshot',
+    lib.st_qk_norm_rope_append.argtypes = [P, P, P, P]
+    lib.st_window_attention.argtypes = [P, P, P, P]
+    lib.st_window_attention_workspace.argtypes = [P, P, ctypes.c_int32, ctypes.c_int32, ctypes.POINTER(ctypes.c_size_t)]
+    for name in ('st_qk_norm_rope_append', 'st_window_attention', 'st_window_attention_workspace',
+                 'st_batch_create', 'st_batch_create_resident', 'st_batch_step', 'st_batch_reset', 'st_batch_snapshot',
                  'st_batch_device_run', 'st_batch_set_eager',
                  'st_runtime_create', 'st_runtime_step', 'st_runtime_reset', 'st_runtime_stop',
                  'st_runtime_snapshot', 'st_runtime_device_trace', 'st_runtime_device_trace_noalloc',
