@@ -291,10 +291,11 @@ struct TileMath {
       return word4_t{pack16<M>(a[0], a[1]), pack16<M>(a[2], a[3]), pack16<M>(b[0], b[1]), pack16<M>(b[2], b[3])};
     }
   }
-  // Tiles that are not seen whole and hold values of V that are not finite: adds such values to the
-  // outputs of the rows that see them, then makes them zeros in LDS, so that the products add nothing.
+  // Tiles that are not seen whole and hold values of V that are not finite: this adds such values to the
+  // outputs of the rows that see them, before clear makes them zeros, which the products then add nothing
+  // for.
   template <int MB, typename Sees>
-  __device__ static __forceinline__ void settle(char* vt, float4_t (&o)[MB][D / 16], int lane, Sees&& sees) {
+  __device__ static __forceinline__ void add_odd(const char* vt, float4_t (&o)[MB][D / 16], int lane, Sees&& sees) {
     const int g = lane >> 4;
 #pragma unroll 1
     for (int r = 0; r < KT; r++) {
@@ -324,9 +325,11 @@ struct TileMath {
         }
       }
     }
-    wave_sync();
+  }
+  template <int kThreads>
+  __device__ static __forceinline__ void clear(char* vt, int thread) {
 #pragma unroll 1
-    for (int at = lane * 16; at < KT * T::kRow; at += 64 * 16) {
+    for (int at = thread * 16; at < KT * T::kRow; at += kThreads * 16) {
       word4_t w = lds_load<word4_t>(vt + at);
 #pragma unroll
       for (int i = 0; i < 4; i++) {
@@ -339,7 +342,23 @@ struct TileMath {
       }
       lds_put(vt + at, w);
     }
-    wave_sync();
+  }
+  // O^T += V^T P^T of the tile.
+  template <int MB>
+  __device__ static __forceinline__ void outputs(const char* vt, const float4_t (&pw)[MB][kBlocks], float4_t (&o)[MB][D / 16],
+                                                 int lane) {
+#pragma unroll
+    for (int depth = 0; depth < kDepths; depth++) {
+      word4_t w[MB];
+#pragma unroll
+      for (int u = 0; u < MB; u++) w[u] = weights(pw[u], depth);
+#pragma unroll
+      for (int d = 0; d < D / 16; d++) {
+        const word4_t v = values(vt, depth, d, lane);
+#pragma unroll
+        for (int u = 0; u < MB; u++) o[u][d] = Mfma<M>::mul(v, w[u], o[u][d]);
+      }
+    }
   }
 };
 
@@ -376,7 +395,7 @@ __device__ __forceinline__ void store_out(const AttentionView& a, int row, int h
 //
 // A masked key's weight is an exact zero, but zero times a value that is not finite is NaN: tiles that are
 // not seen whole look for such values as they are staged, and where there is one they are added apart, for
-// the rows that see them (TileMath::settle).
+// the rows that see them (TileMath::add_odd).
 template <int A, int C, int D, int MB>
 __global__ __launch_bounds__(kAttentionThreads, D == 256 ? 1 : 2) void cache_attention(CacheView c, RowsView r,
                                                                                      AttentionView a) {
@@ -483,9 +502,14 @@ __global__ __launch_bounds__(kAttentionThreads, D == 256 ? 1 : 2) void cache_att
         if (!whole) odd |= not_finite<M>(w);
       });
     }
-    odd = __ballot(odd) != 0;
-    if (tile + kWaves < t1) load((tile + kWaves) * KT);
     wave_sync();
+    if (__ballot(odd)) {
+      X::add_odd(vt, o, lane, [&](int u, int e) { return seen[u](keys, c.window, j0 + e); });
+      wave_sync();
+      X::template clear<64>(vt, lane);
+      wave_sync();
+    }
+    if (tile + kWaves < t1) load((tile + kWaves) * KT);
 
     float4_t s[X::kBlocks][MB];
 #pragma unroll
@@ -507,7 +531,7 @@ __global__ __launch_bounds__(kAttentionThreads, D == 256 ? 1 : 2) void cache_att
       top = pair32_max(pair16_max(top));
       const float safe = top == -INFINITY ? 0.f : top;
       if (__ballot(top != m[u])) {  // rows whose maximum stays have alpha 1
-        const float alpha = __builtin_amdgcn_exp2f(m[u] - safe);
+        const float alpha = m[u] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[u] - safe);  // O may hold infinities
         l[u] *= alpha;
 #pragma unroll
         for (int d = 0; d < D / 16; d++) o[u][d] *= alpha;
@@ -522,19 +546,7 @@ __global__ __launch_bounds__(kAttentionThreads, D == 256 ? 1 : 2) void cache_att
         }
       }
     }
-    if (odd) X::settle(vt, o, lane, [&](int u, int e) { return seen[u](keys, c.window, j0 + e); });
-#pragma unroll
-    for (int depth = 0; depth < X::kDepths; depth++) {
-      word4_t w[MB];
-#pragma unroll
-      for (int u = 0; u < MB; u++) w[u] = X::weights(pw[u], depth);
-#pragma unroll
-      for (int d = 0; d < D / 16; d++) {
-        const word4_t v = X::values(vt, depth, d, lane);
-#pragma unroll
-        for (int u = 0; u < MB; u++) o[u][d] = Mfma<M>::mul(v, w[u], o[u][d]);
-      }
-    }
+    X::outputs(vt, pw, o, lane);
   }
 
   // Merge of the four waves.
@@ -584,6 +596,191 @@ __global__ __launch_bounds__(kAttentionThreads, D == 256 ? 1 : 2) void cache_att
       const float inv = 1.f / sum;
       const float y[4] = {x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
       store_out<A>(a, first + token, h, c.dim, d, y);
+    }
+  }
+}
+
+// Many rows (prompts, long pieces): bound by the matrix products. Workgroup (kv head, row tile; stream):
+// four waves of MB blocks of 16 rows each. The tile of keys is the workgroup's, staged once for its rows:
+// two tiles of LDS, so that one is computed while the next one's loads are in flight in registers, and
+// one barrier per tile. Row tiles of one (stream, kv head) follow each other in the grid at steps of
+// kv_heads, those that see most keys first: with eight heads, or a multiple, each XCD's L2 holds one head's keys.
+constexpr int kRowsThreads = 256;
+template <int M, int D>
+constexpr int rows_tile() {
+  return M == kTF32 ? 4096 / D : D == 256 ? 32 : 64;
+}
+template <int A, int C, int D, int MB>
+__global__ __launch_bounds__(kRowsThreads, D == 256 ? 1 : 2) void cache_attention_rows(CacheView c, RowsView r, AttentionView a) {
+  constexpr int M = mfma_type<A, C>();
+  constexpr int KT = rows_tile<M, D>();
+  using T = TileLayout<M, D>;
+  using R = RowLoad<C, D>;
+  using X = TileMath<M, D, KT>;
+  constexpr int kWaves = kRowsThreads / 64, kRows = kWaves * MB * 16;
+  constexpr int kPerLoad = kRowsThreads / R::L;  // rows of one load of the workgroup
+  constexpr int kLoads = (KT + kPerLoad - 1) / kPerLoad;
+  constexpr int kTile = KT * T::kRow;
+  __shared__ __attribute__((aligned(16))) char lds[2][2][kTile];
+
+  const int head = blockIdx.x % c.kv_heads, b = blockIdx.y;
+  const int64_t start = c.positions[b];
+  int first, n;
+  stream_rows(r, b, first, n);
+  const int rows = n * a.group, tiles_of_rows = (rows + kRows - 1) / kRows;
+  const int tile_of_rows = tiles_of_rows - 1 - (int)(blockIdx.x / c.kv_heads);
+  if (start < 0 || tile_of_rows < 0) return;
+  const int row0 = tile_of_rows * kRows, last_row = min(row0 + kRows, rows) - 1;
+  KeyList keys;
+  keys.init(c, start + row0 / a.group, start + last_row / a.group);
+
+  const int wave = wave_id(), lane = lane_id(), g = lane >> 4;
+  const int p = threadIdx.x % R::L, sub = threadIdx.x / R::L;
+  const bool keep = p * R::E < c.dim;
+  const int64_t base_row = b * c.stream_stride + head * c.head_stride;
+  const char* kbase = c.keys + base_row * c.row_bytes + (keep ? p * 16 : 0);
+  const char* vbase = c.values + base_row * c.row_bytes + (keep ? p * 16 : 0);
+  const int pairs = C == kTInt4 ? c.dim / kQuantGroup : 0;
+  const uint32_t* kpbase = C == kTInt4 ? c.key_params + base_row * pairs + (keep ? p : 0) : nullptr;
+  const uint32_t* vpbase = C == kTInt4 ? c.value_params + base_row * pairs + (keep ? p : 0) : nullptr;
+  const uint32_t slot_bytes = c.slot_stride * c.row_bytes;
+  word4_t kw[kLoads], vw[kLoads];
+  unsigned kp[kLoads], vp[kLoads];
+  auto load = [&](int j0) {
+#pragma unroll
+    for (int i = 0; i < kLoads; i++) {
+      const int slot = keys.slot(min(j0 + min(i * kPerLoad + sub, KT - 1), keys.total - 1));
+      kw[i] = load_global<word4_t>(kbase + (uint64_t)slot * slot_bytes);
+      vw[i] = load_global<word4_t>(vbase + (uint64_t)slot * slot_bytes);
+      if constexpr (C == kTInt4) {
+        const uint64_t at = (uint64_t)slot * c.slot_stride * pairs;
+        kp[i] = load_global<unsigned>(kpbase + at);
+        vp[i] = load_global<unsigned>(vpbase + at);
+      }
+    }
+  };
+  // Stages the loaded tile; look: whether any of its values of V is not finite.
+  auto stage = [&](int buffer, bool look) {
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < kLoads; i++) {
+      const int row = i * kPerLoad + sub;
+      if (KT % kPerLoad != 0 && row >= KT) break;
+      expand<C, M>(kw[i], kp[i], p, keep, [&](int ch, word4_t w) { lds_put(lds[buffer][0] + row * T::kRow + T::key_chunk(row, ch) * 16, w); });
+      expand<C, M>(vw[i], vp[i], p, keep, [&](int ch, word4_t w) {
+        lds_put(lds[buffer][1] + row * T::kRow + T::value_chunk(row, ch) * 16, w);
+        if (look) found |= not_finite<M>(w);
+      });
+    }
+    return found;
+  };
+
+  const int tiles = (keys.total + KT - 1) / KT;
+  load(0);
+  QueryBlock<A, M, D> q[MB];
+  Seen seen[MB];
+  float m[MB], l[MB];
+  float4_t o[MB][D / 16];
+  const int wave_row0 = row0 + wave * MB * 16, wave_last = min(wave_row0 + MB * 16 - 1, last_row);
+#pragma unroll
+  for (int u = 0; u < MB; u++) {
+    const int row = min(wave_row0 + u * 16 + (lane & 15), last_row);
+    const int token = row / a.group, h = head * a.group + row - token * a.group;
+    q[u].load(a.q + (first + token) * a.q_token + h * a.q_head, c.dim, a.scale, g, wave_row0 + u * 16 + (lane & 15) <= last_row);
+    seen[u].init(keys, start + token);
+    m[u] = -INFINITY;
+    l[u] = 0.f;
+#pragma unroll
+    for (int d = 0; d < D / 16; d++) o[u][d] = float4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  // What the wave's rows see of the list: all of them the entries [whole_from, whole_to) of the ring and the
+  // first whole_sinks; some of them nothing of the ring before some_from or from some_to on.
+  const bool idle = wave_row0 > last_row;
+  const int64_t ta = start + min(wave_row0, last_row) / a.group, tb = start + wave_last / a.group;
+  const int newest_a = (int)max(ta - keys.lo, (int64_t)-1), newest_b = (int)max(tb - keys.lo, (int64_t)-1);
+  const int whole_from = keys.sinks + max(newest_b - c.window + 1, 0), whole_to = keys.sinks + newest_a + 1;
+  const int whole_sinks = (int)min((int64_t)keys.sinks, ta + 1);
+  const int some_from = keys.sinks + max(newest_a - c.window + 1, 0), some_to = newest_b < 0 ? (int)min((int64_t)keys.sinks, tb + 1) : keys.sinks + newest_b + 1;
+  // The same of all of the workgroup's rows: tiles that they do not all see whole are looked through for values
+  // that are not finite (cache_attention).
+  const int all_from = keys.sinks + max(keys.total - keys.sinks - c.window, 0);
+  const int all_to = keys.sinks + (int)max(start + row0 / a.group - keys.lo, (int64_t)-1) + 1;
+  auto partial = [&](int j0) { return !(j0 >= all_from && j0 + KT <= all_to); };
+  bool odd = __syncthreads_or(stage(0, partial(0))) != 0;
+
+  for (int tile = 0; tile < tiles; tile++) {
+    const int j0 = tile * KT, buffer = tile & 1;
+    const bool none = idle || j0 >= some_to || (j0 >= keys.sinks && j0 + KT <= some_from);
+    const char* kt = lds[buffer][0];
+    char* vt = lds[buffer][1];
+    if (odd) {
+      if (!none) X::add_odd(vt, o, lane, [&](int u, int e) { return seen[u](keys, c.window, j0 + e); });
+      __syncthreads();
+      X::template clear<kRowsThreads>(vt, threadIdx.x);
+      __syncthreads();
+    }
+    if (tile + 1 < tiles) load(j0 + KT);
+    if (!none) {
+      const bool whole = (j0 >= whole_from && j0 + KT <= whole_to) || j0 + KT <= whole_sinks ||
+                         (whole_sinks == keys.sinks && whole_from == keys.sinks && j0 + KT <= whole_to);
+      float4_t s[X::kBlocks][MB];
+#pragma unroll
+      for (int kb = 0; kb < X::kBlocks; kb++) X::logits(kt, kb, q, s[kb], lane);
+      float4_t pw[MB][X::kBlocks];
+#pragma unroll
+      for (int u = 0; u < MB; u++) {
+        float top = m[u];
+#pragma unroll
+        for (int kb = 0; kb < X::kBlocks; kb++) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            float x = s[kb][u][i] * q[u].factor;
+            if (!whole && !seen[u](keys, c.window, j0 + kb * 16 + g * 4 + i)) x = -INFINITY;
+            pw[u][kb][i] = x;
+            top = fmaxf(top, x);
+          }
+        }
+        top = pair32_max(pair16_max(top));
+        const float safe = top == -INFINITY ? 0.f : top;
+        if (__ballot(top != m[u])) {  // rows whose maximum stays have alpha 1
+          const float alpha = m[u] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[u] - safe);  // O may hold infinities
+          l[u] *= alpha;
+#pragma unroll
+          for (int d = 0; d < D / 16; d++) o[u][d] *= alpha;
+          m[u] = top;
+        }
+#pragma unroll
+        for (int kb = 0; kb < X::kBlocks; kb++) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            pw[u][kb][i] = __builtin_amdgcn_exp2f(pw[u][kb][i] - safe);
+            l[u] += pw[u][kb][i];
+          }
+        }
+      }
+      X::outputs(vt, pw, o, lane);
+    }
+    if (tile + 1 < tiles) {
+      const bool look = partial(j0 + KT), found = stage(buffer ^ 1, look);
+      if (look) odd = __syncthreads_or(found) != 0;
+      else {
+        odd = false;
+        __syncthreads();
+      }
+    }
+  }
+
+#pragma unroll
+  for (int u = 0; u < MB; u++) {
+    const float inv = 1.f / pair32_add(pair16_add(l[u]));
+    const int row = wave_row0 + u * 16 + (lane & 15);
+    if (row <= last_row) {
+      const int token = row / a.group, h = head * a.group + row - token * a.group;
+#pragma unroll
+      for (int d = 0; d < D / 16; d++) {
+        const float y[4] = {o[u][d][0] * inv, o[u][d][1] * inv, o[u][d][2] * inv, o[u][d][3] * inv};
+        if (d * 16 + g * 4 < c.dim) store_out<A>(a, first + token, h, c.dim, d * 16 + g * 4, y);
+      }
     }
   }
 }

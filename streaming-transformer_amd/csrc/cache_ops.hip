@@ -60,17 +60,26 @@ void check_heads(const st_kv_cache* cache, const st_new_rows* rows, int q_heads)
 int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
 struct Plan {
-  int blocks;  // blocks of 16 rows in a workgroup
+  bool many;   // cache_attention_rows, else cache_attention
+  int blocks;  // blocks of 16 rows in a workgroup (many: in a wave)
   int tiles;   // row tiles of a (stream, kv head)
   int splits;
 };
 Plan plan_attention(const CacheView& c, const RowsView& r, int q_heads, int dtype) {
-  Plan p;
+  Plan p{};
   const int rows = r.max_tokens * (q_heads / c.kv_heads), padded = padded_dim(c.dim);
   p.blocks = rows > 16 && padded < 256 ? 2 : 1;  // head dimension 256: one block's registers fill the file
   p.tiles = (rows + 16 * p.blocks - 1) / (16 * p.blocks);
+  const int64_t pairs = (int64_t)c.streams * c.kv_heads;
+  if (rows > 64) {
+    p.many = true;
+    p.blocks = padded == 256 ? 1 : 2;
+    p.tiles = (rows + 64 * p.blocks - 1) / (64 * p.blocks);
+    p.splits = 1;
+    return p;
+  }
   // Workgroups beside the splits, and as many as the chip holds at once (2 per CU; 1 of head dimension 256).
-  const int64_t base = (int64_t)c.streams * c.kv_heads * p.tiles;
+  const int64_t base = pairs * p.tiles;
   const int64_t room = padded == 256 ? 256 : 512;
   const int64_t keys = (int64_t)c.sinks + std::min<int64_t>(c.ring, (int64_t)c.window + r.max_tokens - 1);
   const int64_t share = 4 * 32 * 2;  // fewest keys of a split: two tiles for each wave
@@ -94,6 +103,7 @@ void launch_attention(const CacheView& c, const RowsView& r, const AttentionView
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kAttentionThreads), 0, stream, c, r, a); };
   auto form = [&](auto D) {
     constexpr int d = decltype(D)::value;
+    if (p.many) return go(cache_attention_rows<A, C, d, d == 256 ? 1 : 2>);
     if constexpr (d < 256) {
       if (p.blocks == 2) return go(cache_attention<A, C, d, 2>);
     }
