@@ -340,7 +340,7 @@ int st_qk_norm_rope_append(const st_kv_cache* cache, const st_new_rows* rows, co
                            void* stream);
 
 /* Attention of the new tokens' queries over the cache, which holds their keys and values already:
- * softmax(scale * q . K) V over the positions that a query sees. q_heads is a multiple of
+ * softmax(scale * q . K) V over the positions that a query sees, scale > 0. q_heads is a multiple of
  * kv_heads, and query head h reads cache head h / (q_heads / kv_heads). Strides and types as above.
  * The workspace holds st_window_attention_workspace's bytes (which depend on the structs' numbers
  * alone; 0: none needed) and is 16-byte aligned; its contents matter during the call only. */

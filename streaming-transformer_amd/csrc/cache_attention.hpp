@@ -27,6 +27,11 @@ struct AttentionView {
   int out_ld;
 };
 
+__device__ __forceinline__ int64_t uniform64(int64_t v) {
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 |
+                   (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
+
 // The keys that some query of the tokens ta .. tb (positions) sees, as a list: first the sinks, then the
 // ring's positions lo .. tb. j is an index into the list.
 struct KeyList {
@@ -42,6 +47,12 @@ struct KeyList {
     ring = c.ring;
     slots_sinks = c.sinks;
   }
+  // The slot of entry j if the n entries from it on are consecutive slots, else -1.
+  __device__ __forceinline__ int run(int j, int n) const {
+    int o = offset + j - sinks;
+    o = o >= ring ? o - ring : o;
+    return j >= sinks && j + n <= total && o + n <= ring ? slots_sinks + o : -1;
+  }
   __device__ __forceinline__ int slot(int j) const {
     const int o = offset + j - sinks;
     return j < sinks ? j : slots_sinks + (o >= ring ? o - ring : o);
@@ -54,9 +65,11 @@ struct Seen {
     t = (int)min(position, (int64_t)1 << 30);
     newest = (int)max(position - k.lo, (int64_t)-1);
   }
+  // No short circuits: they compile to a tree of branches for each of a lane's keys.
   __device__ __forceinline__ bool operator()(const KeyList& k, int window, int j) const {
     const int e = j - k.sinks;
-    return j < k.total && (e < 0 ? j <= t : e <= newest && e > newest - window);
+    const bool ringed = (e <= newest) & (e > newest - window), sink = j <= t;
+    return (j < k.total) & ((e < 0) ? sink : ringed);
   }
 };
 
@@ -249,15 +262,15 @@ struct TileMath {
   static constexpr int kBlocks = KT / 16;
   // S^T of one block of 16 keys for each of MB blocks of rows.
   template <int MB, typename Q>
-  __device__ static __forceinline__ void logits(const char* kt, int kb, const Q (&q)[MB], float4_t (&s)[MB], int lane) {
+  __device__ static __forceinline__ void logits(const char* kt, int kb, const Q (&q)[MB], float4_t (&s)[MB][kBlocks], int lane) {
     const int r = kb * 16 + (lane & 15), g = lane >> 4;
 #pragma unroll
-    for (int m = 0; m < MB; m++) s[m] = float4_t{0.f, 0.f, 0.f, 0.f};
+    for (int m = 0; m < MB; m++) s[m][kb] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int step = 0; step < Q::kSteps; step++) {
       const word4_t k = lds_load<word4_t>(kt + r * T::kRow + T::key_chunk(r, step * 4 + g) * 16);
 #pragma unroll
-      for (int m = 0; m < MB; m++) s[m] = Mfma<M>::mul(k, q[m].f[step], s[m]);
+      for (int m = 0; m < MB; m++) s[m][kb] = Mfma<M>::mul(k, q[m].f[step], s[m][kb]);
     }
   }
   // The V operand of 16 dims (block db) and one depth of P: 32 keys (blocks 2 d, 2 d + 1), FP32 16 keys.
@@ -362,6 +375,42 @@ struct TileMath {
   }
 };
 
+// One tile's softmax step for a block of 16 rows: s the products (masked ones -inf), becomes the weights
+// exp2(s * factor - m), whose sum goes to l. m, the maximum that the weights are relative to, moves only when a
+// row's logits pass it by more than 2^8: the weights stay below 256 then, far from any type's limit, and
+// almost every tile is spared the rescaling of O (one that follows every maximum ran for most tiles, as
+// one of 16 rows nearly always has a new one). factor > 0, so the largest product is the largest logit.
+template <int N, int ND>
+__device__ __forceinline__ void softmax_step(float4_t (&s)[N], float factor, float& m, float& l, float4_t (&o)[ND]) {
+  float top = s[0][0];
+#pragma unroll
+  for (int kb = 0; kb < N; kb++) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) top = fmaxf(top, s[kb][i]);
+  }
+  top = pair32_max(pair16_max(top)) * factor;
+  const bool move = top > m + 8.f;  // -inf has no weights yet: any logit passes it
+  if (__ballot(move)) {
+    // O of a row without weights may hold infinities that were added apart: it keeps them.
+    const float alpha = !move || m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
+    l *= alpha;
+#pragma unroll
+    for (int d = 0; d < ND; d++) o[d] *= alpha;
+    m = move ? top : m;
+  }
+  const float base = m == -INFINITY ? 0.f : m;
+  float sum[2] = {0.f, 0.f};
+#pragma unroll
+  for (int kb = 0; kb < N; kb++) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], factor, -base));
+      sum[i & 1] += s[kb][i];
+    }
+  }
+  l += sum[0] + sum[1];
+}
+
 constexpr int kAttentionThreads = 256;  // cache_attention's workgroup: four waves
 
 // Keys of a wave's tile: 16 KB of K and V, or what one MFMA depth needs.
@@ -416,9 +465,11 @@ __global__ __launch_bounds__(kAttentionThreads, D == 256 ? 1 : 2) void cache_att
 
   const int split = blockIdx.x % a.splits, head = blockIdx.x / a.splits % c.kv_heads;
   const int tile_of_rows = blockIdx.x / a.splits / c.kv_heads, b = blockIdx.y;
-  const int64_t start = c.positions[b];
+  const int64_t start = uniform64(c.positions[b]);
   int first, n;
   stream_rows(r, b, first, n);
+  first = __builtin_amdgcn_readfirstlane(first);
+  n = __builtin_amdgcn_readfirstlane(n);
   const int row0 = tile_of_rows * MB * 16, rows = n * a.group;
   if (start < 0 || row0 >= rows) return;
   const int last_row = min(row0 + MB * 16, rows) - 1;
@@ -434,27 +485,51 @@ __global__ __launch_bounds__(kAttentionThreads, D == 256 ? 1 : 2) void cache_att
   const int p = lane % R::L, sub = lane / R::L;
   const bool keep = p * R::E < c.dim;
   const int64_t base_row = b * c.stream_stride + head * c.head_stride;
-  const char* kbase = c.keys + base_row * c.row_bytes + (keep ? p * 16 : 0);
-  const char* vbase = c.values + base_row * c.row_bytes + (keep ? p * 16 : 0);
+  const char* kbase = c.keys + base_row * c.row_bytes;
+  const char* vbase = c.values + base_row * c.row_bytes;
   const int pairs = C == kTInt4 ? c.dim / kQuantGroup : 0;
-  const uint32_t* kpbase = C == kTInt4 ? c.key_params + base_row * pairs + (keep ? p : 0) : nullptr;
-  const uint32_t* vpbase = C == kTInt4 ? c.value_params + base_row * pairs + (keep ? p : 0) : nullptr;
-  const uint32_t slot_bytes = c.slot_stride * c.row_bytes;
+  const uint32_t* kpbase = C == kTInt4 ? c.key_params + base_row * pairs : nullptr;
+  const uint32_t* vpbase = C == kTInt4 ? c.value_params + base_row * pairs : nullptr;
+  const uint32_t slot_bytes = c.slot_stride * c.row_bytes, chunk = keep ? p * 16 : 0, pair = keep ? p : 0;
+  const bool near = slot_bytes < 1u << 25;  // a tile's rows within 32 bits of its first
   word4_t kw[kLoads], vw[kLoads];
   unsigned kp[kLoads], vp[kLoads];
+  const uint32_t run_lane = sub * slot_bytes + chunk, run_pair = sub * c.slot_stride * pairs + pair;
   auto load = [&](int j0) {
+    const int run = near ? keys.run(j0, KT) : -1;
+    if (run >= 0) {  // one slot after the other: the tile's address is the workgroup's, the lane's part stays
+#pragma unroll
+      for (int i = 0; i < kLoads; i++) {
+        const uint64_t at = (uint64_t)(run + i * kPerLoad) * slot_bytes;
+        kw[i] = load_global<word4_t>(kbase + at + run_lane);
+      }
+#pragma unroll
+      for (int i = 0; i < kLoads; i++) {
+        const uint64_t at = (uint64_t)(run + i * kPerLoad) * slot_bytes;
+        vw[i] = load_global<word4_t>(vbase + at + run_lane);
+      }
+      if constexpr (C == kTInt4) {
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) {
+          const uint64_t at = (uint64_t)(run + i * kPerLoad) * c.slot_stride * pairs;
+          kp[i] = load_global<unsigned>(kpbase + at + run_pair);
+          vp[i] = load_global<unsigned>(vpbase + at + run_pair);
+        }
+      }
+      return;
+    }
     int slot[kLoads];
 #pragma unroll
     for (int i = 0; i < kLoads; i++) {
       slot[i] = keys.slot(min(j0 + i * kPerLoad + sub, keys.total - 1));
-      kw[i] = load_global<word4_t>(kbase + (uint64_t)slot[i] * slot_bytes);
+      kw[i] = load_global<word4_t>(kbase + (uint64_t)slot[i] * slot_bytes + chunk);
     }
 #pragma unroll
-    for (int i = 0; i < kLoads; i++) vw[i] = load_global<word4_t>(vbase + (uint64_t)slot[i] * slot_bytes);
+    for (int i = 0; i < kLoads; i++) vw[i] = load_global<word4_t>(vbase + (uint64_t)slot[i] * slot_bytes + chunk);
     if constexpr (C == kTInt4) {
 #pragma unroll
       for (int i = 0; i < kLoads; i++) {
-        const uint64_t at = (uint64_t)slot[i] * c.slot_stride * pairs;
+        const uint64_t at = (uint64_t)slot[i] * c.slot_stride * pairs + pair;
         kp[i] = load_global<unsigned>(kpbase + at);
         vp[i] = load_global<unsigned>(vpbase + at);
       }
@@ -511,42 +586,24 @@ __global__ __launch_bounds__(kAttentionThreads, D == 256 ? 1 : 2) void cache_att
     }
     if (tile + kWaves < t1) load((tile + kWaves) * KT);
 
-    float4_t s[X::kBlocks][MB];
+    float4_t s[MB][X::kBlocks];
 #pragma unroll
-    for (int kb = 0; kb < X::kBlocks; kb++) X::logits(kt, kb, q, s[kb], lane);
-    float4_t pw[MB][X::kBlocks];
+    for (int kb = 0; kb < X::kBlocks; kb++) X::logits(kt, kb, q, s, lane);
 #pragma unroll
     for (int u = 0; u < MB; u++) {
-      float top = m[u];
+      if (!whole) {
 #pragma unroll
-      for (int kb = 0; kb < X::kBlocks; kb++) {
+        for (int kb = 0; kb < X::kBlocks; kb++) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          float x = s[kb][u][i] * q[u].factor;
-          if (!whole && !seen[u](keys, c.window, j0 + kb * 16 + g * 4 + i)) x = -INFINITY;
-          pw[u][kb][i] = x;
-          top = fmaxf(top, x);
+          for (int i = 0; i < 4; i++) {
+            const float x = s[u][kb][i];
+            s[u][kb][i] = seen[u](keys, c.window, j0 + kb * 16 + g * 4 + i) ? x : -INFINITY;
+          }
         }
       }
-      top = pair32_max(pair16_max(top));
-      const float safe = top == -INFINITY ? 0.f : top;
-      if (__ballot(top != m[u])) {  // rows whose maximum stays have alpha 1
-        const float alpha = m[u] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[u] - safe);  // O may hold infinities
-        l[u] *= alpha;
-#pragma unroll
-        for (int d = 0; d < D / 16; d++) o[u][d] *= alpha;
-        m[u] = top;
-      }
-#pragma unroll
-      for (int kb = 0; kb < X::kBlocks; kb++) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          pw[u][kb][i] = __builtin_amdgcn_exp2f(pw[u][kb][i] - safe);
-          l[u] += pw[u][kb][i];
-        }
-      }
+      softmax_step(s[u], q[u].factor, m[u], l[u], o[u]);
     }
-    X::outputs(vt, pw, o, lane);
+    X::outputs(vt, s, o, lane);
   }
 
   // Merge of the four waves.
@@ -624,9 +681,11 @@ __global__ __launch_bounds__(kRowsThreads, D == 256 ? 1 : 2) void cache_attentio
   __shared__ __attribute__((aligned(16))) char lds[2][2][kTile];
 
   const int head = blockIdx.x % c.kv_heads, b = blockIdx.y;
-  const int64_t start = c.positions[b];
+  const int64_t start = uniform64(c.positions[b]);
   int first, n;
   stream_rows(r, b, first, n);
+  first = __builtin_amdgcn_readfirstlane(first);
+  n = __builtin_amdgcn_readfirstlane(n);
   const int rows = n * a.group, tiles_of_rows = (rows + kRows - 1) / kRows;
   const int tile_of_rows = tiles_of_rows - 1 - (int)(blockIdx.x / c.kv_heads);
   if (start < 0 || tile_of_rows < 0) return;
@@ -638,22 +697,39 @@ __global__ __launch_bounds__(kRowsThreads, D == 256 ? 1 : 2) void cache_attentio
   const int p = threadIdx.x % R::L, sub = threadIdx.x / R::L;
   const bool keep = p * R::E < c.dim;
   const int64_t base_row = b * c.stream_stride + head * c.head_stride;
-  const char* kbase = c.keys + base_row * c.row_bytes + (keep ? p * 16 : 0);
-  const char* vbase = c.values + base_row * c.row_bytes + (keep ? p * 16 : 0);
+  const char* kbase = c.keys + base_row * c.row_bytes;
+  const char* vbase = c.values + base_row * c.row_bytes;
   const int pairs = C == kTInt4 ? c.dim / kQuantGroup : 0;
-  const uint32_t* kpbase = C == kTInt4 ? c.key_params + base_row * pairs + (keep ? p : 0) : nullptr;
-  const uint32_t* vpbase = C == kTInt4 ? c.value_params + base_row * pairs + (keep ? p : 0) : nullptr;
-  const uint32_t slot_bytes = c.slot_stride * c.row_bytes;
+  const uint32_t* kpbase = C == kTInt4 ? c.key_params + base_row * pairs : nullptr;
+  const uint32_t* vpbase = C == kTInt4 ? c.value_params + base_row * pairs : nullptr;
+  const uint32_t slot_bytes = c.slot_stride * c.row_bytes, chunk = keep ? p * 16 : 0, pair = keep ? p : 0;
+  const bool near = slot_bytes < 1u << 25;  // a tile's rows within 32 bits of its first
   word4_t kw[kLoads], vw[kLoads];
   unsigned kp[kLoads], vp[kLoads];
+  const uint32_t run_lane = min(sub, KT - 1) * slot_bytes + chunk, run_pair = min(sub, KT - 1) * c.slot_stride * pairs + pair;
   auto load = [&](int j0) {
+    const int run = near ? keys.run(j0, KT) : -1;
+    if (run >= 0) {
+#pragma unroll
+      for (int i = 0; i < kLoads; i++) {
+        const uint64_t at = (uint64_t)(run + i * kPerLoad) * slot_bytes;
+        kw[i] = load_global<word4_t>(kbase + at + run_lane);
+        vw[i] = load_global<word4_t>(vbase + at + run_lane);
+        if constexpr (C == kTInt4) {
+          const uint64_t pat = (uint64_t)(run + i * kPerLoad) * c.slot_stride * pairs;
+          kp[i] = load_global<unsigned>(kpbase + pat + run_pair);
+          vp[i] = load_global<unsigned>(vpbase + pat + run_pair);
+        }
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < kLoads; i++) {
       const int slot = keys.slot(min(j0 + min(i * kPerLoad + sub, KT - 1), keys.total - 1));
-      kw[i] = load_global<word4_t>(kbase + (uint64_t)slot * slot_bytes);
-      vw[i] = load_global<word4_t>(vbase + (uint64_t)slot * slot_bytes);
+      kw[i] = load_global<word4_t>(kbase + (uint64_t)slot * slot_bytes + chunk);
+      vw[i] = load_global<word4_t>(vbase + (uint64_t)slot * slot_bytes + chunk);
       if constexpr (C == kTInt4) {
-        const uint64_t at = (uint64_t)slot * c.slot_stride * pairs;
+        const uint64_t at = (uint64_t)slot * c.slot_stride * pairs + pair;
         kp[i] = load_global<unsigned>(kpbase + at);
         vp[i] = load_global<unsigned>(vpbase + at);
       }
@@ -723,42 +799,24 @@ __global__ __launch_bounds__(kRowsThreads, D == 256 ? 1 : 2) void cache_attentio
     if (!none) {
       const bool whole = (j0 >= whole_from && j0 + KT <= whole_to) || j0 + KT <= whole_sinks ||
                          (whole_sinks == keys.sinks && whole_from == keys.sinks && j0 + KT <= whole_to);
-      float4_t s[X::kBlocks][MB];
+      float4_t s[MB][X::kBlocks];
 #pragma unroll
-      for (int kb = 0; kb < X::kBlocks; kb++) X::logits(kt, kb, q, s[kb], lane);
-      float4_t pw[MB][X::kBlocks];
+      for (int kb = 0; kb < X::kBlocks; kb++) X::logits(kt, kb, q, s, lane);
 #pragma unroll
       for (int u = 0; u < MB; u++) {
-        float top = m[u];
+        if (!whole) {
 #pragma unroll
-        for (int kb = 0; kb < X::kBlocks; kb++) {
+          for (int kb = 0; kb < X::kBlocks; kb++) {
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            float x = s[kb][u][i] * q[u].factor;
-            if (!whole && !seen[u](keys, c.window, j0 + kb * 16 + g * 4 + i)) x = -INFINITY;
-            pw[u][kb][i] = x;
-            top = fmaxf(top, x);
+            for (int i = 0; i < 4; i++) {
+              const float x = s[u][kb][i];
+              s[u][kb][i] = seen[u](keys, c.window, j0 + kb * 16 + g * 4 + i) ? x : -INFINITY;
+            }
           }
         }
-        top = pair32_max(pair16_max(top));
-        const float safe = top == -INFINITY ? 0.f : top;
-        if (__ballot(top != m[u])) {  // rows whose maximum stays have alpha 1
-          const float alpha = m[u] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[u] - safe);  // O may hold infinities
-          l[u] *= alpha;
-#pragma unroll
-          for (int d = 0; d < D / 16; d++) o[u][d] *= alpha;
-          m[u] = top;
-        }
-#pragma unroll
-        for (int kb = 0; kb < X::kBlocks; kb++) {
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            pw[u][kb][i] = __builtin_amdgcn_exp2f(pw[u][kb][i] - safe);
-            l[u] += pw[u][kb][i];
-          }
-        }
+        softmax_step(s[u], q[u].factor, m[u], l[u], o[u]);
       }
-      X::outputs(vt, pw, o, lane);
+      X::outputs(vt, s, o, lane);
     }
     if (tile + 1 < tiles) {
       const bool look = partial(j0 + KT), found = stage(buffer ^ 1, look);

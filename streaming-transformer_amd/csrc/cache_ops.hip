@@ -253,7 +253,7 @@ void attend_rows(const st_kv_cache* cache, const st_new_rows* rows, const st_att
   require(args != nullptr, "Null argument");
   check_types(args->dtype, cache->dtype);
   check_heads(cache, rows, args->q_heads);
-  require(std::isfinite(args->scale), "The scale must be finite");
+  require(std::isfinite(args->scale) && args->scale > 0, "The scale must be positive and finite");
   if (r.tokens == 0) return;
   AttentionView a{};
   a.q = static_cast<const char*>(args->q);

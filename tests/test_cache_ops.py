@@ -112,6 +112,7 @@ def test_append_arguments_refused(change, match):
     (dict(q=None), 'Null'), (dict(out=None), 'Null'), (dict(q=A + 8), 'multiples of 16'), (dict(out=A + 4), 'multiples of 16'),
     (dict(out_strides=(256, 3)), 'multiples of 16'), (dict(out_strides=(0, 64)), 'overlap'),
     (dict(scale=float('nan')), 'scale'), (dict(scale=float('inf')), 'scale'),
+    (dict(scale=0.0), 'scale'), (dict(scale=-0.125), 'scale'),
 ], ids=str)
 def test_attention_arguments_refused(change, match):
     refused(cache(), rows(), attention_args(**change), match)
