@@ -11,6 +11,8 @@
 
 #include "cache_device.hpp"
 
+#include <type_traits>
+
 namespace stamd {
 
 struct AttentionView {
@@ -47,11 +49,21 @@ struct KeyList {
     ring = c.ring;
     slots_sinks = c.sinks;
   }
-  // The slot of entry j if the n entries from it on are consecutive slots, else -1.
-  __device__ __forceinline__ int run(int j, int n) const {
-    int o = offset + j - sinks;
+  // Offsets of n rows, `step` apart, of the `count` entries from j0 on: in units of slots, row i of the lane at entry
+  // min(j0 + min(i * step + sub, count - 1), total - 1). Where the entries are consecutive slots, and their
+  // offsets within 32 bits of the first (near), the lane's part `part` = sub * unit is given.
+  template <int N>
+  __device__ __forceinline__ void offsets(int j0, int step, int sub, int count, bool near, uint32_t unit, uint32_t part,
+                                          uint64_t (&at)[N]) const {
+    int o = offset + j0 - sinks;
     o = o >= ring ? o - ring : o;
-    return j >= sinks && j + n <= total && o + n <= ring ? slots_sinks + o : -1;
+    if (near && j0 >= sinks && j0 + count <= total && o + count <= ring) {
+#pragma unroll
+      for (int i = 0; i < N; i++) at[i] = (uint64_t)(slots_sinks + o + i * step) * unit + part;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i++) at[i] = (uint64_t)slot(min(j0 + min(i * step + sub, count - 1), total - 1)) * unit;
+    }
   }
   __device__ __forceinline__ int slot(int j) const {
     const int o = offset + j - sinks;
@@ -195,6 +207,12 @@ __device__ __forceinline__ word2_t lds_column4(const char* p) {
   return __builtin_bit_cast(word2_t,
                             __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)p));
 }
+// 16 bytes per lane straight to LDS, lane i's to to + 16 i (`to` is the wave's), and the wait for such loads.
+__device__ __forceinline__ void load_to_lds(const char* from, char* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                   (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
@@ -260,17 +278,32 @@ template <int M, int D, int KT>
 struct TileMath {
   using T = TileLayout<M, D>;
   static constexpr int kBlocks = KT / 16;
-  // S^T of one block of 16 keys for each of MB blocks of rows.
+  // S^T of the tile for MB blocks of rows. Each depth's products go over all blocks: independent sums.
   template <int MB, typename Q>
-  __device__ static __forceinline__ void logits(const char* kt, int kb, const Q (&q)[MB], float4_t (&s)[MB][kBlocks], int lane) {
-    const int r = kb * 16 + (lane & 15), g = lane >> 4;
-#pragma unroll
-    for (int m = 0; m < MB; m++) s[m][kb] = float4_t{0.f, 0.f, 0.f, 0.f};
+  __device__ static __forceinline__ void logits(const char* kt, const Q (&q)[MB], float4_t (&s)[MB][kBlocks], int lane) {
+    const int g = lane >> 4;
 #pragma unroll
     for (int step = 0; step < Q::kSteps; step++) {
-      const word4_t k = lds_load<word4_t>(kt + r * T::kRow + T::key_chunk(r, step * 4 + g) * 16);
 #pragma unroll
-      for (int m = 0; m < MB; m++) s[m][kb] = Mfma<M>::mul(k, q[m].f[step], s[m][kb]);
+      for (int kb = 0; kb < kBlocks; kb++) {
+        const int r = kb * 16 + (lane & 15);
+        const word4_t k = lds_load<word4_t>(kt + r * T::kRow + T::key_chunk(r, step * 4 + g) * 16);
+#pragma unroll
+        for (int u = 0; u < MB; u++)
+          s[u][kb] = Mfma<M>::mul(k, q[u].f[step], step == 0 ? float4_t{0.f, 0.f, 0.f, 0.f} : s[u][kb]);
+      }
+    }
+    // Six reads ahead of the products, then one per MB of them: left alone, the compiler waits for most reads
+    // where it makes them (a prompt of 8192 tokens 271 -> 267 us).
+    if constexpr (M != kTF32 && MB > 1) {
+      constexpr int kReads = Q::kSteps * kBlocks, kAhead = kReads < 6 ? kReads : 6;
+      __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+      for (int i = 0; i < kReads - kAhead; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x8, MB, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x8, MB * kAhead, 0);
     }
   }
   // The V operand of 16 dims (block db) and one depth of P: 32 keys (blocks 2 d, 2 d + 1), FP32 16 keys.
@@ -295,20 +328,11 @@ struct TileMath {
     }
   }
   static constexpr int kDepth = M == kTF32 ? 16 : 32, kDepths = KT / kDepth;
-  // The operand P^T of one depth from the blocks' weights p[block][i].
-  __device__ static __forceinline__ word4_t weights(const float4_t (&p)[kBlocks], int depth) {
-    if constexpr (M == kTF32) {
-      return __builtin_bit_cast(word4_t, p[depth]);
-    } else {
-      const float4_t a = p[2 * depth], b = p[2 * depth + 1];
-      return word4_t{pack16<M>(a[0], a[1]), pack16<M>(a[2], a[3]), pack16<M>(b[0], b[1]), pack16<M>(b[2], b[3])};
-    }
-  }
   // Tiles that are not seen whole and hold values of V that are not finite: this adds such values to the
   // outputs of the rows that see them, before clear makes them zeros, which the products then add nothing
   // for.
   template <int MB, typename Sees>
-  __device__ static __forceinline__ void add_odd(const char* vt, float4_t (&o)[MB][D / 16], int lane, Sees&& sees) {
+  __device__ static __forceinline__ void add_odd(const char* vt, float4_t (&o)[MB][D / 16 + 1], int lane, Sees&& sees) {
     const int g = lane >> 4;
 #pragma unroll 1
     for (int r = 0; r < KT; r++) {
@@ -356,15 +380,31 @@ struct TileMath {
       lds_put(vt + at, w);
     }
   }
-  // O^T += V^T P^T of the tile.
-  template <int MB>
-  __device__ static __forceinline__ void outputs(const char* vt, const float4_t (&pw)[MB][kBlocks], float4_t (&o)[MB][D / 16],
-                                                 int lane) {
+  // O^T += V^T P^T of the tile, P = exp2(s factor - base), each depth's weights made right before its products. The
+  // last block of O is the rows' sums: for 16-bit products those of the rounded weights, by a product with
+  // ones (every element is the row's whole sum), for FP32 the lane's own share in four parts.
+  template <int MB, typename Q>
+  __device__ static __forceinline__ void outputs(const char* vt, const float4_t (&s)[MB][kBlocks], const Q (&q)[MB],
+                                                 const float (&base)[MB], float4_t (&o)[MB][D / 16 + 1], int lane) {
 #pragma unroll
     for (int depth = 0; depth < kDepths; depth++) {
       word4_t w[MB];
 #pragma unroll
-      for (int u = 0; u < MB; u++) w[u] = weights(pw[u], depth);
+      for (int u = 0; u < MB; u++) {
+        float p[kDepth / 4];
+#pragma unroll
+        for (int i = 0; i < kDepth / 4; i++)
+          p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][depth * (kDepth / 16) + i / 4][i % 4], q[u].factor, -base[u]));
+        if constexpr (M == kTF32) {
+          const float4_t x = {p[0], p[1], p[2], p[3]};
+          w[u] = __builtin_bit_cast(word4_t, x);
+          o[u][D / 16] += x;
+        } else {
+          constexpr unsigned one = M == kTF16 ? 0x3c003c00u : 0x3f803f80u;
+          w[u] = word4_t{pack16<M>(p[0], p[1]), pack16<M>(p[2], p[3]), pack16<M>(p[4], p[5]), pack16<M>(p[6], p[7])};
+          o[u][D / 16] = Mfma<M>::mul(word4_t{one, one, one, one}, w[u], o[u][D / 16]);
+        }
+      }
 #pragma unroll
       for (int d = 0; d < D / 16; d++) {
         const word4_t v = values(vt, depth, d, lane);
@@ -373,42 +413,77 @@ struct TileMath {
       }
     }
   }
-};
-
-// One tile's softmax step for a block of 16 rows: s the products (masked ones -inf), becomes the weights
-// exp2(s * factor - m), whose sum goes to l. m, the maximum that the weights are relative to, moves only when a
-// row's logits pass it by more than 2^8: the weights stay below 256 then, far from any type's limit, and
-// almost every tile is spared the rescaling of O (one that follows every maximum ran for most tiles, as
-// one of 16 rows nearly always has a new one). factor > 0, so the largest product is the largest logit.
-template <int N, int ND>
-__device__ __forceinline__ void softmax_step(float4_t (&s)[N], float factor, float& m, float& l, float4_t (&o)[ND]) {
-  float top = s[0][0];
-#pragma unroll
-  for (int kb = 0; kb < N; kb++) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) top = fmaxf(top, s[kb][i]);
+  // A row's sum of weights, from the last block of its O.
+  __device__ static __forceinline__ float row_sum(const float4_t& x) {
+    if constexpr (M == kTF32) return pair32_add(pair16_add((x[0] + x[1]) + (x[2] + x[3])));
+    else return x[0];
   }
-  top = pair32_max(pair16_max(top)) * factor;
-  const bool move = top > m + 8.f;  // -inf has no weights yet: any logit passes it
-  if (__ballot(move)) {
-    // O of a row without weights may hold infinities that were added apart: it keeps them.
-    const float alpha = !move || m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
-    l *= alpha;
+  // Entries that a row does not see: minus infinity.
+  template <int MB, typename See>
+  __device__ static __forceinline__ void mask(float4_t (&s)[MB][kBlocks], const See (&seen)[MB], const KeyList& keys, int window,
+                                              int j0, int lane) {
+    const int j = j0 + (lane >> 4) * 4;
 #pragma unroll
-    for (int d = 0; d < ND; d++) o[d] *= alpha;
-    m = move ? top : m;
-  }
-  const float base = m == -INFINITY ? 0.f : m;
-  float sum[2] = {0.f, 0.f};
+    for (int u = 0; u < MB; u++) {
+      if (j0 >= keys.sinks) {
+        const int age = seen[u].newest + keys.sinks - j;
 #pragma unroll
-  for (int kb = 0; kb < N; kb++) {
+        for (int kb = 0; kb < kBlocks; kb++) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], factor, -base));
-      sum[i & 1] += s[kb][i];
+          for (int i = 0; i < 4; i++) {
+            const float x = s[u][kb][i];
+            s[u][kb][i] = (unsigned)(age - kb * 16 - i) < (unsigned)window ? x : -INFINITY;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int kb = 0; kb < kBlocks; kb++) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const float x = s[u][kb][i];
+            s[u][kb][i] = seen[u](keys, window, j + kb * 16 + i) ? x : -INFINITY;
+          }
+        }
+      }
     }
   }
-  l += sum[0] + sum[1];
+};
+
+// The maxima m that the weights exp2(s factor - m) of MB blocks of 16 rows are relative to, s a tile's products
+// (masked ones -inf). A row's moves only when its logits pass it by more than 2^8: the weights stay below 256
+// then, far from any type's limit, and almost every tile is spared the rescaling of O (one that follows every
+// maximum ran for most tiles, as one of 16 rows nearly always has a new one: a prompt of 8192 tokens 360 -> 320 us
+// together with the scaling inside the exponential). factor > 0, so the largest product is the largest logit.
+// base: m, or 0 for rows without a logit so far.
+template <int MB, int N, int ND, typename Q>
+__device__ __forceinline__ void move_maxima(const float4_t (&s)[MB][N], const Q (&q)[MB], float (&m)[MB], float (&base)[MB],
+                                            float4_t (&o)[MB][ND]) {
+  float top[MB];
+  bool any = false;
+#pragma unroll
+  for (int u = 0; u < MB; u++) {
+    top[u] = s[u][0][0];
+#pragma unroll
+    for (int kb = 0; kb < N; kb++) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) top[u] = fmaxf(top[u], s[u][kb][i]);
+    }
+    top[u] = pair32_max(pair16_max(top[u])) * q[u].factor;
+    any |= top[u] > m[u] + 8.f;  // -inf has no weights yet: any logit passes it
+  }
+  if (__ballot(any)) {
+#pragma unroll
+    for (int u = 0; u < MB; u++) {
+      const bool move = top[u] > m[u] + 8.f;
+      // O of a row without weights may hold infinities that were added apart: it keeps them.
+      const float alpha = !move || m[u] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[u] - top[u]);
+#pragma unroll
+      for (int d = 0; d < ND; d++) o[u][d] *= alpha;
+      m[u] = move ? top[u] : m[u];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < MB; u++) base[u] = m[u] == -INFINITY ? 0.f : m[u];
 }
 
 constexpr int kAttentionThreads = 256;  // cache_attention's workgroup: four waves
@@ -487,51 +562,28 @@ __global__ __launch_bounds__(kAttentionThreads, D == 256 ? 1 : 2) void cache_att
   const int64_t base_row = b * c.stream_stride + head * c.head_stride;
   const char* kbase = c.keys + base_row * c.row_bytes;
   const char* vbase = c.values + base_row * c.row_bytes;
-  const int pairs = C == kTInt4 ? c.dim / kQuantGroup : 0;
-  const uint32_t* kpbase = C == kTInt4 ? c.key_params + base_row * pairs : nullptr;
-  const uint32_t* vpbase = C == kTInt4 ? c.value_params + base_row * pairs : nullptr;
+  const char* kpbase = C == kTInt4 ? reinterpret_cast<const char*>(c.key_params) + base_row * (c.row_bytes / 4) : nullptr;
+  const char* vpbase = C == kTInt4 ? reinterpret_cast<const char*>(c.value_params) + base_row * (c.row_bytes / 4) : nullptr;
   const uint32_t slot_bytes = c.slot_stride * c.row_bytes, chunk = keep ? p * 16 : 0, pair = keep ? p : 0;
   const bool near = slot_bytes < 1u << 25;  // a tile's rows within 32 bits of its first
   word4_t kw[kLoads], vw[kLoads];
   unsigned kp[kLoads], vp[kLoads];
-  const uint32_t run_lane = sub * slot_bytes + chunk, run_pair = sub * c.slot_stride * pairs + pair;
+  // The loads have one place and no condition: a branch around them, or two forms of them, makes the compiler
+  // move what they return, which waits for it. Those past the last tile repeat it.
+  const uint32_t part = sub * slot_bytes;
   auto load = [&](int j0) {
-    const int run = near ? keys.run(j0, KT) : -1;
-    if (run >= 0) {  // one slot after the other: the tile's address is the workgroup's, the lane's part stays
+    uint64_t at[kLoads];
+    keys.offsets(j0, kPerLoad, sub, KT, near, slot_bytes, part, at);
 #pragma unroll
-      for (int i = 0; i < kLoads; i++) {
-        const uint64_t at = (uint64_t)(run + i * kPerLoad) * slot_bytes;
-        kw[i] = load_global<word4_t>(kbase + at + run_lane);
-      }
+    for (int i = 0; i < kLoads; i++) kw[i] = load_global<word4_t>(kbase + at[i] + chunk);
 #pragma unroll
-      for (int i = 0; i < kLoads; i++) {
-        const uint64_t at = (uint64_t)(run + i * kPerLoad) * slot_bytes;
-        vw[i] = load_global<word4_t>(vbase + at + run_lane);
-      }
-      if constexpr (C == kTInt4) {
-#pragma unroll
-        for (int i = 0; i < kLoads; i++) {
-          const uint64_t at = (uint64_t)(run + i * kPerLoad) * c.slot_stride * pairs;
-          kp[i] = load_global<unsigned>(kpbase + at + run_pair);
-          vp[i] = load_global<unsigned>(vpbase + at + run_pair);
-        }
-      }
-      return;
-    }
-    int slot[kLoads];
-#pragma unroll
-    for (int i = 0; i < kLoads; i++) {
-      slot[i] = keys.slot(min(j0 + i * kPerLoad + sub, keys.total - 1));
-      kw[i] = load_global<word4_t>(kbase + (uint64_t)slot[i] * slot_bytes + chunk);
-    }
-#pragma unroll
-    for (int i = 0; i < kLoads; i++) vw[i] = load_global<word4_t>(vbase + (uint64_t)slot[i] * slot_bytes + chunk);
+    for (int i = 0; i < kLoads; i++) vw[i] = load_global<word4_t>(vbase + at[i] + chunk);
     if constexpr (C == kTInt4) {
 #pragma unroll
       for (int i = 0; i < kLoads; i++) {
-        const uint64_t at = (uint64_t)slot[i] * c.slot_stride * pairs + pair;
-        kp[i] = load_global<unsigned>(kpbase + at);
-        vp[i] = load_global<unsigned>(vpbase + at);
+        const uint64_t params = at[i] / 16 * 4 + pair * 4;  // 16 bytes of codes have 4 of scale and minimum
+        kp[i] = load_global<unsigned>(kpbase + params);
+        vp[i] = load_global<unsigned>(vpbase + params);
       }
     }
   };
@@ -539,12 +591,12 @@ __global__ __launch_bounds__(kAttentionThreads, D == 256 ? 1 : 2) void cache_att
   const int tiles = (keys.total + KT - 1) / KT, per = (tiles + a.splits - 1) / a.splits;
   const int t1 = min((split + 1) * per, tiles);
   int tile = split * per + wave;
-  if (tile < t1) load(tile * KT);
+  load(min(tile, tiles - 1) * KT);
 
   QueryBlock<A, M, D> q[MB];
   Seen seen[MB];
-  float m[MB], l[MB];
-  float4_t o[MB][D / 16];
+  float m[MB];
+  float4_t o[MB][D / 16 + 1];  // and the sums of the weights
 #pragma unroll
   for (int u = 0; u < MB; u++) {
     const int row = min(row0 + u * 16 + (lane & 15), last_row);
@@ -552,9 +604,8 @@ __global__ __launch_bounds__(kAttentionThreads, D == 256 ? 1 : 2) void cache_att
     q[u].load(a.q + (first + token) * a.q_token + h * a.q_head, c.dim, a.scale, g, row0 + u * 16 + (lane & 15) <= last_row);
     seen[u].init(keys, start + token);
     m[u] = -INFINITY;
-    l[u] = 0.f;
 #pragma unroll
-    for (int d = 0; d < D / 16; d++) o[u][d] = float4_t{0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d <= D / 16; d++) o[u][d] = float4_t{0.f, 0.f, 0.f, 0.f};
   }
   // List entries that every row sees: from whole_from on, up to whole_to (ring entries).
   const int whole_from = keys.sinks + max((int)(tb - keys.lo) - c.window + 1, 0);
@@ -584,35 +635,23 @@ __global__ __launch_bounds__(kAttentionThreads, D == 256 ? 1 : 2) void cache_att
       X::template clear<64>(vt, lane);
       wave_sync();
     }
-    if (tile + kWaves < t1) load((tile + kWaves) * KT);
+    load(min(tile + kWaves, t1 - 1) * KT);
 
     float4_t s[MB][X::kBlocks];
-#pragma unroll
-    for (int kb = 0; kb < X::kBlocks; kb++) X::logits(kt, kb, q, s, lane);
-#pragma unroll
-    for (int u = 0; u < MB; u++) {
-      if (!whole) {
-#pragma unroll
-        for (int kb = 0; kb < X::kBlocks; kb++) {
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const float x = s[u][kb][i];
-            s[u][kb][i] = seen[u](keys, c.window, j0 + kb * 16 + g * 4 + i) ? x : -INFINITY;
-          }
-        }
-      }
-      softmax_step(s[u], q[u].factor, m[u], l[u], o[u]);
-    }
-    X::outputs(vt, s, o, lane);
+    float base[MB];
+    X::logits(kt, q, s, lane);
+    if (!whole) X::mask(s, seen, keys, c.window, j0, lane);
+    move_maxima(s, q, m, base, o);
+    X::outputs(vt, s, q, base, o, lane);
   }
 
   // Merge of the four waves.
 #pragma unroll
   for (int u = 0; u < MB; u++) {
-    l[u] = pair32_add(pair16_add(l[u]));
+    const float l = X::row_sum(o[u][D / 16]);
     if (g == 0) {
       ml[wave][0][u * 16 + (lane & 15)] = m[u];
-      ml[wave][1][u * 16 + (lane & 15)] = l[u];
+      ml[wave][1][u * 16 + (lane & 15)] = l;
     }
   }
   __syncthreads();
@@ -659,8 +698,8 @@ __global__ __launch_bounds__(kAttentionThreads, D == 256 ? 1 : 2) void cache_att
 
 // Many rows (prompts, long pieces): bound by the matrix products. Workgroup (kv head, row tile; stream):
 // four waves of MB blocks of 16 rows each. The tile of keys is the workgroup's, staged once for its rows:
-// two tiles of LDS, so that one is computed while the next one's loads are in flight in registers, and
-// one barrier per tile. Row tiles of one (stream, kv head) follow each other in the grid at steps of
+// two tiles of LDS, so that one is computed while the next one's loads are in flight (straight to LDS where the
+// rows need no conversion), and one barrier per tile. Row tiles of one (stream, kv head) follow each other in the grid at steps of
 // kv_heads, those that see most keys first: with eight heads, or a multiple, each XCD's L2 holds one head's keys.
 constexpr int kRowsThreads = 256;
 template <int M, int D>
@@ -678,6 +717,8 @@ __global__ __launch_bounds__(kRowsThreads, D == 256 ? 1 : 2) void cache_attentio
   constexpr int kPerLoad = kRowsThreads / R::L;  // rows of one load of the workgroup
   constexpr int kLoads = (KT + kPerLoad - 1) / kPerLoad;
   constexpr int kTile = KT * T::kRow;
+  constexpr bool kDirect = C == M;
+  static_assert(!kDirect || KT % kPerLoad == 0);
   __shared__ __attribute__((aligned(16))) char lds[2][2][kTile];
 
   const int head = blockIdx.x % c.kv_heads, b = blockIdx.y;
@@ -693,70 +734,80 @@ __global__ __launch_bounds__(kRowsThreads, D == 256 ? 1 : 2) void cache_attentio
   KeyList keys;
   keys.init(c, start + row0 / a.group, start + last_row / a.group);
 
-  const int wave = wave_id(), lane = lane_id(), g = lane >> 4;
   const int p = threadIdx.x % R::L, sub = threadIdx.x / R::L;
   const bool keep = p * R::E < c.dim;
   const int64_t base_row = b * c.stream_stride + head * c.head_stride;
   const char* kbase = c.keys + base_row * c.row_bytes;
   const char* vbase = c.values + base_row * c.row_bytes;
-  const int pairs = C == kTInt4 ? c.dim / kQuantGroup : 0;
-  const uint32_t* kpbase = C == kTInt4 ? c.key_params + base_row * pairs : nullptr;
-  const uint32_t* vpbase = C == kTInt4 ? c.value_params + base_row * pairs : nullptr;
+  const char* kpbase = C == kTInt4 ? reinterpret_cast<const char*>(c.key_params) + base_row * (c.row_bytes / 4) : nullptr;
+  const char* vpbase = C == kTInt4 ? reinterpret_cast<const char*>(c.value_params) + base_row * (c.row_bytes / 4) : nullptr;
   const uint32_t slot_bytes = c.slot_stride * c.row_bytes, chunk = keep ? p * 16 : 0, pair = keep ? p : 0;
   const bool near = slot_bytes < 1u << 25;  // a tile's rows within 32 bits of its first
   word4_t kw[kLoads], vw[kLoads];
   unsigned kp[kLoads], vp[kLoads];
-  const uint32_t run_lane = min(sub, KT - 1) * slot_bytes + chunk, run_pair = min(sub, KT - 1) * c.slot_stride * pairs + pair;
-  auto load = [&](int j0) {
-    const int run = near ? keys.run(j0, KT) : -1;
-    if (run >= 0) {
+  const uint32_t part = min(sub, KT - 1) * slot_bytes;
+  const int wave = wave_id(), lane = lane_id(), g = lane >> 4;
+  // The loads of the tile at entry j0: rows that need no conversion go straight to LDS, others to registers.
+  auto load = [&](int j0, int buffer) {
+    uint64_t at[kLoads];
+    keys.offsets(j0, kPerLoad, sub, KT, near, slot_bytes, part, at);
+    if constexpr (kDirect) {
+      // A wave's load fills 64 consecutive chunks of the tile: the lane fetches the one that belongs there.
 #pragma unroll
       for (int i = 0; i < kLoads; i++) {
-        const uint64_t at = (uint64_t)(run + i * kPerLoad) * slot_bytes;
-        kw[i] = load_global<word4_t>(kbase + at + run_lane);
-        vw[i] = load_global<word4_t>(vbase + at + run_lane);
-        if constexpr (C == kTInt4) {
-          const uint64_t pat = (uint64_t)(run + i * kPerLoad) * c.slot_stride * pairs;
-          kp[i] = load_global<unsigned>(kpbase + pat + run_pair);
-          vp[i] = load_global<unsigned>(vpbase + pat + run_pair);
-        }
+        const int row = i * kPerLoad + sub, to = (i * kRowsThreads + wave * 64) * 16;
+        const int kc = T::key_chunk(row, p), vc = T::value_chunk(row, p);
+        if (kc * R::E < c.dim) load_to_lds(kbase + at[i] + kc * 16, lds[buffer][0] + to);
+        if (vc * R::E < c.dim) load_to_lds(vbase + at[i] + vc * 16, lds[buffer][1] + to);
       }
-      return;
-    }
+    } else {
 #pragma unroll
-    for (int i = 0; i < kLoads; i++) {
-      const int slot = keys.slot(min(j0 + min(i * kPerLoad + sub, KT - 1), keys.total - 1));
-      kw[i] = load_global<word4_t>(kbase + (uint64_t)slot * slot_bytes + chunk);
-      vw[i] = load_global<word4_t>(vbase + (uint64_t)slot * slot_bytes + chunk);
-      if constexpr (C == kTInt4) {
-        const uint64_t at = (uint64_t)slot * c.slot_stride * pairs + pair;
-        kp[i] = load_global<unsigned>(kpbase + at);
-        vp[i] = load_global<unsigned>(vpbase + at);
+      for (int i = 0; i < kLoads; i++) {
+        kw[i] = load_global<word4_t>(kbase + at[i] + chunk);
+        vw[i] = load_global<word4_t>(vbase + at[i] + chunk);
+        if constexpr (C == kTInt4) {
+          const uint64_t params = at[i] / 16 * 4 + pair * 4;  // 16 bytes of codes have 4 of scale and minimum
+          kp[i] = load_global<unsigned>(kpbase + params);
+          vp[i] = load_global<unsigned>(vpbase + params);
+        }
       }
     }
   };
-  // Stages the loaded tile; look: whether any of its values of V is not finite.
+  // Waits for the loads and stages what came to registers; look: whether any value of V is not finite.
   auto stage = [&](int buffer, bool look) {
     bool found = false;
+    if constexpr (kDirect) {
+      wait_loads();
+      if (look) {
 #pragma unroll
-    for (int i = 0; i < kLoads; i++) {
-      const int row = i * kPerLoad + sub;
-      if (KT % kPerLoad != 0 && row >= KT) break;
-      expand<C, M>(kw[i], kp[i], p, keep, [&](int ch, word4_t w) { lds_put(lds[buffer][0] + row * T::kRow + T::key_chunk(row, ch) * 16, w); });
-      expand<C, M>(vw[i], vp[i], p, keep, [&](int ch, word4_t w) {
-        lds_put(lds[buffer][1] + row * T::kRow + T::value_chunk(row, ch) * 16, w);
-        if (look) found |= not_finite<M>(w);
-      });
+        for (int i = 0; i < kLoads; i++)
+          found |= not_finite<M>(lds_load<word4_t>(lds[buffer][1] + (i * kRowsThreads + (int)threadIdx.x) * 16));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kLoads; i++) {
+        const int row = i * kPerLoad + sub;
+        if (KT % kPerLoad != 0 && row >= KT) break;
+        expand<C, M>(kw[i], kp[i], p, keep, [&](int ch, word4_t w) { lds_put(lds[buffer][0] + row * T::kRow + T::key_chunk(row, ch) * 16, w); });
+        expand<C, M>(vw[i], vp[i], p, keep, [&](int ch, word4_t w) {
+          lds_put(lds[buffer][1] + row * T::kRow + T::value_chunk(row, ch) * 16, w);
+          if (look) found |= not_finite<M>(w);
+        });
+      }
     }
     return found;
   };
+  if (kDirect && c.dim < D) {  // the padding, which no load writes
+    for (int at = threadIdx.x * 16; at < 4 * kTile; at += kRowsThreads * 16) lds_put(&lds[0][0][0] + at, word4_t{0, 0, 0, 0});
+    __syncthreads();
+  }
 
   const int tiles = (keys.total + KT - 1) / KT;
-  load(0);
+  load(0, 0);
   QueryBlock<A, M, D> q[MB];
   Seen seen[MB];
-  float m[MB], l[MB];
-  float4_t o[MB][D / 16];
+  float m[MB];
+  float4_t o[MB][D / 16 + 1];  // and the sums of the weights
   const int wave_row0 = row0 + wave * MB * 16, wave_last = min(wave_row0 + MB * 16 - 1, last_row);
 #pragma unroll
   for (int u = 0; u < MB; u++) {
@@ -765,58 +816,48 @@ __global__ __launch_bounds__(kRowsThreads, D == 256 ? 1 : 2) void cache_attentio
     q[u].load(a.q + (first + token) * a.q_token + h * a.q_head, c.dim, a.scale, g, wave_row0 + u * 16 + (lane & 15) <= last_row);
     seen[u].init(keys, start + token);
     m[u] = -INFINITY;
-    l[u] = 0.f;
 #pragma unroll
-    for (int d = 0; d < D / 16; d++) o[u][d] = float4_t{0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d <= D / 16; d++) o[u][d] = float4_t{0.f, 0.f, 0.f, 0.f};
   }
-  // What the wave's rows see of the list: all of them the entries [whole_from, whole_to) of the ring and the
-  // first whole_sinks; some of them nothing of the ring before some_from or from some_to on.
+  // What some of the wave's rows see of the ring's entries: nothing before some_from or from some_to on.
   const bool idle = wave_row0 > last_row;
   const int64_t ta = start + min(wave_row0, last_row) / a.group, tb = start + wave_last / a.group;
   const int newest_a = (int)max(ta - keys.lo, (int64_t)-1), newest_b = (int)max(tb - keys.lo, (int64_t)-1);
-  const int whole_from = keys.sinks + max(newest_b - c.window + 1, 0), whole_to = keys.sinks + newest_a + 1;
-  const int whole_sinks = (int)min((int64_t)keys.sinks, ta + 1);
-  const int some_from = keys.sinks + max(newest_a - c.window + 1, 0), some_to = newest_b < 0 ? (int)min((int64_t)keys.sinks, tb + 1) : keys.sinks + newest_b + 1;
-  // The same of all of the workgroup's rows: tiles that they do not all see whole are looked through for values
+  const int some_from = keys.sinks + max(newest_a - c.window + 1, 0);
+  const int some_to = newest_b < 0 ? (int)min((int64_t)keys.sinks, tb + 1) : keys.sinks + newest_b + 1;
+  // All of the workgroup's rows see the entries [all_from, all_to). Other tiles are looked through for values
   // that are not finite (cache_attention).
   const int all_from = keys.sinks + max(keys.total - keys.sinks - c.window, 0);
   const int all_to = keys.sinks + (int)max(start + row0 / a.group - keys.lo, (int64_t)-1) + 1;
   auto partial = [&](int j0) { return !(j0 >= all_from && j0 + KT <= all_to); };
   bool odd = __syncthreads_or(stage(0, partial(0))) != 0;
 
-  for (int tile = 0; tile < tiles; tile++) {
+  // One tile. kWhole: all of the workgroup's rows see all of it.
+  auto step = [&](int tile, auto kWhole) {
     const int j0 = tile * KT, buffer = tile & 1;
-    const bool none = idle || j0 >= some_to || (j0 >= keys.sinks && j0 + KT <= some_from);
     const char* kt = lds[buffer][0];
     char* vt = lds[buffer][1];
-    if (odd) {
-      if (!none) X::add_odd(vt, o, lane, [&](int u, int e) { return seen[u](keys, c.window, j0 + e); });
-      __syncthreads();
-      X::template clear<kRowsThreads>(vt, threadIdx.x);
-      __syncthreads();
-    }
-    if (tile + 1 < tiles) load(j0 + KT);
-    if (!none) {
-      const bool whole = (j0 >= whole_from && j0 + KT <= whole_to) || j0 + KT <= whole_sinks ||
-                         (whole_sinks == keys.sinks && whole_from == keys.sinks && j0 + KT <= whole_to);
-      float4_t s[MB][X::kBlocks];
-#pragma unroll
-      for (int kb = 0; kb < X::kBlocks; kb++) X::logits(kt, kb, q, s, lane);
-#pragma unroll
-      for (int u = 0; u < MB; u++) {
-        if (!whole) {
-#pragma unroll
-          for (int kb = 0; kb < X::kBlocks; kb++) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-              const float x = s[u][kb][i];
-              s[u][kb][i] = seen[u](keys, c.window, j0 + kb * 16 + g * 4 + i) ? x : -INFINITY;
-            }
-          }
-        }
-        softmax_step(s[u], q[u].factor, m[u], l[u], o[u]);
+    bool none = false;
+    if constexpr (!kWhole) {
+      none = idle || j0 >= some_to || (j0 >= keys.sinks && j0 + KT <= some_from);
+      if (odd) {
+        if (!none) X::add_odd(vt, o, lane, [&](int u, int e) { return seen[u](keys, c.window, j0 + e); });
+        __syncthreads();
+        X::template clear<kRowsThreads>(vt, threadIdx.x);
+        __syncthreads();
       }
-      X::outputs(vt, s, o, lane);
+    }
+    float4_t s[MB][X::kBlocks];
+    float base[MB];
+    if (!none) X::logits(kt, q, s, lane);
+    // The next tile's loads, after the reads of K: the compiler lets no LDS read pass a load to LDS before it has
+    // arrived, and the next ones are V's, behind the maxima. Loads to registers have no condition around them, and
+    // repeat the last tile: with one, or in two forms, the compiler moves what they return and waits for it.
+    if (!kDirect || tile + 1 < tiles) load(min(tile + 1, tiles - 1) * KT, buffer ^ 1);
+    if (!none) {
+      if constexpr (!kWhole) X::mask(s, seen, keys, c.window, j0, lane);
+      move_maxima(s, q, m, base, o);
+      X::outputs(vt, s, q, base, o, lane);
     }
     if (tile + 1 < tiles) {
       const bool look = partial(j0 + KT), found = stage(buffer ^ 1, look);
@@ -826,11 +867,20 @@ __global__ __launch_bounds__(kRowsThreads, D == 256 ? 1 : 2) void cache_attentio
         __syncthreads();
       }
     }
+  };
+  // The tiles seen whole are one run: a loop of their own, in which nothing branches around the products (a
+  // branch around the masks alone cost a register move per logit).
+  const int run_from = min((all_from + KT - 1) / KT, tiles), run_to = max(run_from, all_to / KT);
+  int tile = 0;
+  for (int round = 0; round < 2; round++) {
+    const int until = round ? tiles : run_from;
+    for (; tile < until; tile++) step(tile, std::false_type{});
+    for (; tile < run_to; tile++) step(tile, std::true_type{});
   }
 
 #pragma unroll
   for (int u = 0; u < MB; u++) {
-    const float inv = 1.f / pair32_add(pair16_add(l[u]));
+    const float inv = 1.f / X::row_sum(o[u][D / 16]);
     const int row = wave_row0 + u * 16 + (lane & 15);
     if (row <= last_row) {
       const int token = row / a.group, h = head * a.group + row - token * a.group;
