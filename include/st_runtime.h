@@ -315,8 +315,8 @@ typedef struct {
   const int32_t* offsets;
 } st_new_rows;
 
-/* Norm of each query and key head (x / sqrt(mean(x^2) + epsilon) * gain; none where the gain is
- * NULL), rotation of its first rope_dims elements by the token's angles, and the append of keys and
+/* Norm of each query and key head (x / sqrt(mean(x^2) + epsilon) * gain, epsilon at least 1e-37; none where
+ * the gain is NULL), rotation of its first rope_dims elements by the token's angles, and the append of keys and
  * values to the cache, in one pass. Element (2i, 2i + 1) pairs, or (i, i + rope_dims / 2) with
  * rope_halves, are rotated by position * inv_freq[i] radians, or by the rotation (cos, sin) at
  * rope[(row * rope_dims / 2 + i) * 2]: one of the two must be given where rope_dims > 0.

@@ -213,11 +213,6 @@ __device__ __forceinline__ void load_to_lds(const char* from, char* to) {
                                    (__attribute__((address_space(3))) void*)to, 16, 0, 0);
 }
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-__device__ __forceinline__ void wave_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
 
 // The type that the MFMAs take: FP32 for FP32 queries (every cache type widens to it exactly), else the
 // queries' own; 4-bit rows become FP16 for bfloat16 queries too, whose eight significant bits FP16 holds

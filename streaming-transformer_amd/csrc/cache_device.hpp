@@ -103,6 +103,13 @@ __device__ __forceinline__ float high16(unsigned u) {
   else return bits_to_float(u & 0xffff0000u);
 }
 
+// Orders a wave's LDS accesses among its lanes.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Eight consecutive elements of type T (FP32, FP16 or bfloat16) as loaded, and as FP32 values.
 template <int T>
 struct Eight {

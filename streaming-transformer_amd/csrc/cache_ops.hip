@@ -92,9 +92,13 @@ size_t workspace_of(const CacheView& c, const RowsView& r, int q_heads, const Pl
   return (size_t)c.streams * q_heads * r.max_tokens * p.splits * (8 + (size_t)c.dim * 4);
 }
 
+// Tokens from which a wave takes one, else a workgroup.
+constexpr int kWaveTokens = 1024;
+
 template <int A, int C>
 void launch_append(const CacheView& c, const RowsView& r, const AppendView& a, hipStream_t stream) {
-  hipLaunchKernelGGL((cache_append<A, C>), dim3(r.tokens), dim3(kAppendThreads), 0, stream, c, r, a);
+  if (r.tokens < kWaveTokens) hipLaunchKernelGGL((cache_append<A, C, 256>), dim3(r.tokens), dim3(kAppendThreads), 0, stream, c, r, a);
+  else hipLaunchKernelGGL((cache_append<A, C, 64>), dim3((r.tokens + 3) / 4), dim3(kAppendThreads), 0, stream, c, r, a);
 }
 
 template <int A, int C>
@@ -221,7 +225,8 @@ void append_rows(const st_kv_cache* cache, const st_new_rows* rows, const st_app
   a.q_gain = args->q_gain;
   a.k_gain = args->k_gain;
   a.epsilon = args->epsilon;
-  require((!a.q_gain && !a.k_gain) || (std::isfinite(a.epsilon) && a.epsilon > 0), "A norm needs a positive epsilon");
+  require((!a.q_gain && !a.k_gain) || (std::isfinite(a.epsilon) && a.epsilon >= 1e-37f), "A norm needs an epsilon of at least 1e-37");
+  a.inv_dim = 1.f / (float)c.dim;
   a.q_heads = args->q_heads;
   a.rope_dims = args->rope_dims;
   require(a.rope_dims >= 0 && a.rope_dims <= c.dim && a.rope_dims % 2 == 0,

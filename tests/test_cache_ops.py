@@ -98,7 +98,7 @@ def test_rows_refused(change, match):
     (dict(q=A + 4), 'multiples of 16'), (dict(k=A + 8), 'multiples of 16'), (dict(q_out=A + 8), 'multiples of 16'),
     (dict(q_strides=(510, 64)), 'multiples of 16'), (dict(v_strides=(512, 66)), 'multiples of 16'),
     (dict(k_strides=(2**40, 64)), 'Stride'), (dict(out_strides=(0, 64)), 'overlap'), (dict(out_strides=(256, 0)), 'overlap'),
-    (dict(q_gain=A, epsilon=0.0), 'epsilon'), (dict(k_gain=A, epsilon=-1.0), 'epsilon'),
+    (dict(q_gain=A, epsilon=0.0), 'epsilon'), (dict(k_gain=A, epsilon=-1.0), 'epsilon'), (dict(k_gain=A, epsilon=1e-40), 'epsilon'),
     (dict(k_gain=A, epsilon=float('nan')), 'epsilon'), (dict(q_gain=A, epsilon=float('inf')), 'epsilon'),
     (dict(rope_dims=66), 'Rotated'), (dict(rope_dims=31), 'Rotated'), (dict(rope_dims=-2), 'Rotated'),
     (dict(rope_halves=2), 'rope_halves'), (dict(inv_freq=None), 'frequencies'), (dict(rope=A), 'frequencies'),
