@@ -481,8 +481,6 @@ __device__ __forceinline__ void move_maxima(const float4_t (&s)[MB][N], const Q 
   for (int u = 0; u < MB; u++) base[u] = m[u] == -INFINITY ? 0.f : m[u];
 }
 
-constexpr int kAttentionThreads = 256;  // cache_attention's workgroup: four waves
-
 // Keys of a wave's tile: 16 KB of K and V, or what one MFMA depth needs.
 template <int M, int D>
 constexpr int wave_tile() {
@@ -515,15 +513,13 @@ __device__ __forceinline__ void store_out(const AttentionView& a, int row, int h
 // A masked key's weight is an exact zero, but zero times a value that is not finite is NaN: tiles that are
 // not seen whole look for such values as they are staged, and where there is one they are added apart, for
 // the rows that see them (TileMath::add_odd).
-template <int A, int C, int D, int MB>
-__global__ __launch_bounds__(kAttentionThreads, D == 256 ? 1 : 2) void cache_attention(CacheView c, RowsView r,
-                                                                                     AttentionView a) {
+template <int A, int C, int D, int MB, int kWaves>
+__global__ __launch_bounds__(64 * kWaves, 2 * 4 / kWaves) void cache_attention(CacheView c, RowsView r, AttentionView a) {
   constexpr int M = mfma_type<A, C>();
   constexpr int KT = wave_tile<M, D>();
   using T = TileLayout<M, D>;
   using R = RowLoad<C, D>;
   using X = TileMath<M, D, KT>;
-  constexpr int kWaves = kAttentionThreads / 64;
   constexpr int kPerLoad = 64 / R::L;                                // rows of one load of the wave
   constexpr int kLoads = (KT + kPerLoad - 1) / kPerLoad;
   static_assert(KT % kPerLoad == 0);
@@ -666,7 +662,7 @@ __global__ __launch_bounds__(kAttentionThreads, D == 256 ? 1 : 2) void cache_att
   }
   __syncthreads();
   const int quads = c.dim / 4;
-  for (int i = threadIdx.x; i < (last_row - row0 + 1) * quads; i += kAttentionThreads) {
+  for (int i = threadIdx.x; i < (last_row - row0 + 1) * quads; i += 64 * kWaves) {
     const int row = i / quads, d = (i - row * quads) * 4;
     float top = ml[0][0][row], sum = 0.f;
 #pragma unroll
@@ -687,6 +683,232 @@ __global__ __launch_bounds__(kAttentionThreads, D == 256 ? 1 : 2) void cache_att
       const float inv = 1.f / sum;
       const float y[4] = {x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
       store_out<A>(a, first + token, h, c.dim, d, y);
+    }
+  }
+}
+
+// One new token per stream with FP32 queries, at most four query heads per cache head: products of so few rows
+// would leave most of an FP32 MFMA's 16 idle (a step of 16 streams over a 4-bit cache 15.7 us, bound by them),
+// so they are made by vector instructions, without LDS in the loop. A row of the cache is shared by L lanes, E
+// elements each; every group of L lanes takes keys of its own, with its own (m, l, O), and the groups and
+// waves are merged at the end. Each load's registers are loaded again as soon as they are used.
+template <int C, int D>
+constexpr int vector_loads() {  // loads of K (and of V) in flight per wave
+  return C == kTInt4 ? 2 : 8;
+}
+constexpr int kVectorWaves = 8;
+template <int C, int D, int R>
+__global__ __launch_bounds__(64 * kVectorWaves) void cache_attention_vector(CacheView c, RowsView r, AttentionView a) {
+  using Row = RowLoad<C, D>;
+  constexpr int E = Row::E, L = Row::L, kGroups = 64 / L, NB = vector_loads<C, D>(), KT = NB * kGroups;
+  constexpr int kWaves = kVectorWaves;
+  __shared__ __attribute__((aligned(16))) float merge[kWaves][R][D];
+  __shared__ float ml[kWaves][2][R];
+  const int split = blockIdx.x % a.splits, head = blockIdx.x / a.splits, b = blockIdx.y;
+  const int64_t start = uniform64(c.positions[b]);
+  int first, n;
+  stream_rows(r, b, first, n);
+  first = __builtin_amdgcn_readfirstlane(first);
+  n = __builtin_amdgcn_readfirstlane(n);
+  if (start < 0 || n == 0) return;
+  KeyList keys;
+  keys.init(c, start, start);
+  const int wave = wave_id(), lane = lane_id(), p = lane % L, sub = lane / L;
+  const bool keep = p * E < c.dim;
+  const int64_t base_row = b * c.stream_stride + head * c.head_stride;
+  const uint32_t slot_bytes = c.slot_stride * c.row_bytes, chunk = keep ? p * 16 : 0, part = sub * slot_bytes;
+  const bool near = slot_bytes < 1u << 25;
+  const char* const kbase = c.keys + base_row * c.row_bytes + chunk;
+  const char* const vbase = c.values + base_row * c.row_bytes + chunk;
+  const int64_t pbase = C == kTInt4 ? base_row * (c.row_bytes / 4) + (keep ? p * 4 : 0) : 0;
+  const char* const kpbase = reinterpret_cast<const char*>(c.key_params) + pbase;
+  const char* const vpbase = reinterpret_cast<const char*>(c.value_params) + pbase;
+
+  // The queries' elements that meet this lane's.
+  float q[R][E];
+#pragma unroll
+  for (int u = 0; u < R; u++) {
+    const char* row = a.q + first * a.q_token + (head * a.group + min(u, a.group - 1)) * a.q_head + (keep ? p * E * 4 : 0);
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+      const float4_t x = load_global<float4_t>(row + e * 4);
+#pragma unroll
+      for (int i = 0; i < 4; i++) q[u][e + i] = keep ? x[i] * a.scale : 0.f;
+    }
+  }
+  word4_t kw[NB], vw[NB];
+  unsigned kp[NB], vp[NB];
+  uint64_t at[NB];
+  auto load_keys = [&] {
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+      kw[i] = load_global<word4_t>(kbase + at[i]);
+      if constexpr (C == kTInt4) kp[i] = load_global<unsigned>(kpbase + at[i] / 16 * 4);
+    }
+  };
+  auto load_values = [&] {
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+      vw[i] = load_global<word4_t>(vbase + at[i]);
+      if constexpr (C == kTInt4) vp[i] = load_global<unsigned>(vpbase + at[i] / 16 * 4);
+    }
+  };
+  // The elements of a load.
+  auto widen = [&](word4_t w, unsigned params, float (&x)[E]) {
+    if constexpr (C == kTF32) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[i] = bits_to_float(w[i]);
+    } else if constexpr (C == kTInt4) {
+      const half2_t sz = __builtin_bit_cast(half2_t, params);
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        float4_t f[2];
+        dequant8_f32(w[i], (float)sz[0], (float)sz[1], f);
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[8 * i + e] = f[e >> 2][e & 3];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        x[2 * i] = low16<C>(w[i]);
+        x[2 * i + 1] = high16<C>(w[i]);
+      }
+    }
+  };
+
+  const int tiles = (keys.total + KT - 1) / KT, per = (tiles + a.splits - 1) / a.splits;
+  const int t1 = min((split + 1) * per, tiles);
+  int tile = split * per + wave;
+  keys.offsets(min(tile, tiles - 1) * KT, kGroups, sub, KT, near, slot_bytes, part, at);
+  load_keys();
+  load_values();
+  float m[R], l[R], o[R][E];
+#pragma unroll
+  for (int u = 0; u < R; u++) {
+    m[u] = -INFINITY;
+    l[u] = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; e++) o[u][e] = 0.f;
+  }
+  for (; tile < t1; tile += kWaves) {
+    const int j0 = tile * KT;
+    // Entries past the end (of the last tile) weigh nothing, and their loads' repeated rows count as zeros.
+    const bool whole = j0 + KT <= keys.total;
+    keys.offsets(min(tile + kWaves, t1 - 1) * KT, kGroups, sub, KT, near, slot_bytes, part, at);
+    float s[R][NB];
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+      float x[E];
+      widen(kw[i], kp[i], x);
+#pragma unroll
+      for (int u = 0; u < R; u++) {
+        float d[2] = {0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < E; e++) d[e & 1] = __builtin_fmaf(q[u][e], x[e], d[e & 1]);
+        s[u][i] = group_sum(d[0] + d[1], L);
+      }
+    }
+    load_keys();
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < NB; i++) {
+        const bool in = j0 + i * kGroups + sub < keys.total;
+#pragma unroll
+        for (int u = 0; u < R; u++) {
+          const float x = s[u][i];
+          s[u][i] = in ? x : -INFINITY;
+        }
+#pragma unroll
+        for (int w = 0; w < 4; w++) vw[i][w] = in ? vw[i][w] : 0u;
+        if constexpr (C == kTInt4) vp[i] = in ? vp[i] : 0u;
+      }
+    }
+    float top[R], base[R];
+    bool any = false;
+#pragma unroll
+    for (int u = 0; u < R; u++) {
+      top[u] = s[u][0];
+#pragma unroll
+      for (int i = 1; i < NB; i++) top[u] = fmaxf(top[u], s[u][i]);
+      any |= top[u] > m[u] + 8.f;
+    }
+    if (__ballot(any)) {  // as in move_maxima
+#pragma unroll
+      for (int u = 0; u < R; u++) {
+        const bool move = top[u] > m[u] + 8.f;
+        const float alpha = !move || m[u] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[u] - top[u]);
+        l[u] *= alpha;
+#pragma unroll
+        for (int e = 0; e < E; e++) o[u][e] *= alpha;
+        m[u] = move ? top[u] : m[u];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < R; u++) {
+      base[u] = m[u] == -INFINITY ? 0.f : m[u];
+#pragma unroll
+      for (int i = 0; i < NB; i++) {
+        s[u][i] = __builtin_amdgcn_exp2f(s[u][i] - base[u]);
+        l[u] += s[u][i];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+      float x[E];
+      widen(vw[i], vp[i], x);
+#pragma unroll
+      for (int u = 0; u < R; u++) {
+#pragma unroll
+        for (int e = 0; e < E; e++) o[u][e] = __builtin_fmaf(s[u][i], x[e], o[u][e]);
+      }
+    }
+    load_values();
+  }
+
+  // The wave's groups, then the waves.
+#pragma unroll
+  for (int u = 0; u < R; u++) {
+    float top = m[u];
+#pragma unroll
+    for (int x = L; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+    const float f = m[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[u] - top);
+    float sum = m[u] == -INFINITY ? l[u] : l[u] * f;
+#pragma unroll
+    for (int x = L; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      float y = o[u][e] * f;
+#pragma unroll
+      for (int x = L; x < 64; x <<= 1) y += __shfl_xor(y, x);
+      if (sub == 0) merge[wave][u][p * E + e] = y;
+    }
+    if (lane == 0) {
+      ml[wave][0][u] = top;
+      ml[wave][1][u] = sum;
+    }
+  }
+  __syncthreads();
+  const int quads = c.dim / 4;
+  for (int i = threadIdx.x; i < a.group * quads; i += 64 * kWaves) {
+    const int u = i / quads, d = (i - u * quads) * 4;
+    float top = ml[0][0][u], sum = 0.f;
+#pragma unroll
+    for (int w = 1; w < kWaves; w++) top = fmaxf(top, ml[w][0][u]);
+    float4_t x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) {
+      const float mw = ml[w][0][u], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - top);
+      sum += mw == -INFINITY ? ml[w][1][u] : ml[w][1][u] * f;
+      x += *(const float4_t*)(&merge[w][u][d]) * f;
+    }
+    if (a.splits > 1) {
+      const size_t to = (((size_t)b * c.kv_heads + head) * a.rows + u) * a.splits + split;
+      if (d == 0) a.part_ml[to] = make_float2(top, sum);
+      store_global(a.part_o + to * c.dim + d, x);
+    } else {
+      const float inv = 1.f / sum;
+      const float y[4] = {x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
+      store_out<kTF32>(a, first, head * a.group + u, c.dim, d, y);
     }
   }
 }

@@ -60,12 +60,14 @@ void check_heads(const st_kv_cache* cache, const st_new_rows* rows, int q_heads)
 int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
 struct Plan {
-  bool many;   // cache_attention_rows, else cache_attention
+  bool many;   // cache_attention_rows
+  int vector;  // rows of cache_attention_vector; 0, and not many: cache_attention
   int blocks;  // blocks of 16 rows in a workgroup (many: in a wave)
+  int waves;   // of a workgroup
   int tiles;   // row tiles of a (stream, kv head)
   int splits;
 };
-Plan plan_attention(const CacheView& c, const RowsView& r, int q_heads, int dtype) {
+Plan plan_attention(const CacheView& c, const RowsView& r, int q_heads, int dtype, int stored) {
   Plan p{};
   const int rows = r.max_tokens * (q_heads / c.kv_heads), padded = padded_dim(c.dim);
   p.blocks = rows > 16 && padded < 256 ? 2 : 1;  // head dimension 256: one block's registers fill the file
@@ -78,11 +80,15 @@ Plan plan_attention(const CacheView& c, const RowsView& r, int q_heads, int dtyp
     p.splits = 1;
     return p;
   }
+  const int group = q_heads / c.kv_heads;
+  // Four query heads over 4-bit rows, 32 elements of each to a lane, do not fit into registers.
+  if (dtype == ST_TYPE_F32 && r.max_tokens == 1 && group <= (stored == ST_TYPE_INT4 ? 2 : 4)) p.vector = group == 3 ? 4 : group;
   // Workgroups beside the splits, and as many as the chip holds at once (2 per CU; 1 of head dimension 256).
   const int64_t base = pairs * p.tiles;
-  const int64_t room = padded == 256 ? 256 : 512;
+  p.waves = p.vector || (p.blocks == 1 && padded < 256) ? 8 : 4;
+  const int64_t room = padded == 256 || p.waves == 8 ? 256 : 512;
   const int64_t keys = (int64_t)c.sinks + std::min<int64_t>(c.ring, (int64_t)c.window + r.max_tokens - 1);
-  const int64_t share = 4 * 32 * 2;  // fewest keys of a split: two tiles for each wave
+  const int64_t share = p.waves * 32 * 2;  // fewest keys of a split: two tiles for each wave
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(room + base - 1) / base, keys / share, kMaxSplits}));
   return p;
 }
@@ -104,14 +110,22 @@ void launch_append(const CacheView& c, const RowsView& r, const AppendView& a, h
 template <int A, int C>
 void launch_attention(const CacheView& c, const RowsView& r, const AttentionView& a, const Plan& p, hipStream_t stream) {
   const dim3 grid((unsigned)(p.splits * c.kv_heads * p.tiles), c.streams);
-  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kAttentionThreads), 0, stream, c, r, a); };
+  auto go = [&](auto kernel, int threads) { hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, stream, c, r, a); };
   auto form = [&](auto D) {
     constexpr int d = decltype(D)::value;
-    if (p.many) return go(cache_attention_rows<A, C, d, d == 256 ? 1 : 2>);
-    if constexpr (d < 256) {
-      if (p.blocks == 2) return go(cache_attention<A, C, d, 2>);
+    if (p.many) return go(cache_attention_rows<A, C, d, d == 256 ? 1 : 2>, kRowsThreads);
+    if constexpr (A == kTF32) {
+      if (p.vector == 1) return go(cache_attention_vector<C, d, 1>, 64 * kVectorWaves);
+      if (p.vector == 2) return go(cache_attention_vector<C, d, 2>, 64 * kVectorWaves);
+      if constexpr (C != kTInt4) {
+        if (p.vector == 4) return go(cache_attention_vector<C, d, 4>, 64 * kVectorWaves);
+      }
     }
-    go(cache_attention<A, C, d, 1>);
+    if constexpr (d < 256) {
+      if (p.blocks == 2) return go(cache_attention<A, C, d, 2, 4>, 256);
+      if (p.waves == 8) return go(cache_attention<A, C, d, 1, 8>, 512);
+    }
+    go(cache_attention<A, C, d, 1, 4>, 256);
   };
   const int padded = padded_dim(c.dim);
   if (padded == 64) form(std::integral_constant<int, 64>{});
@@ -248,7 +262,7 @@ size_t attention_workspace(const st_kv_cache* cache, const st_new_rows* rows, in
   const RowsView r = rows_view(cache, rows);
   check_types(dtype, cache->dtype);
   check_heads(cache, rows, q_heads);
-  return workspace_of(c, r, q_heads, plan_attention(c, r, q_heads, dtype));
+  return workspace_of(c, r, q_heads, plan_attention(c, r, q_heads, dtype, cache->dtype));
 }
 
 void attend_rows(const st_kv_cache* cache, const st_new_rows* rows, const st_attention_args* args, hipStream_t stream,
@@ -271,7 +285,7 @@ void attend_rows(const st_kv_cache* cache, const st_new_rows* rows, const st_att
   a.rows = r.max_tokens * a.group;
   a.out_layout = out_layout;
   a.out_ld = out_ld;
-  const Plan p = plan_attention(c, r, args->q_heads, args->dtype);
+  const Plan p = plan_attention(c, r, args->q_heads, args->dtype, cache->dtype);
   a.splits = p.splits;
   const size_t need = workspace_of(c, r, args->q_heads, p);
   if (need) {

@@ -50,11 +50,12 @@ class _Attention(ctypes.Structure):
 
 _torch = None
 _types = {}
+_stream = None  # device index -> torch's current stream, a hipStream_t
 
 
 def _load():
     """torch and the library, sharing one HIP runtime."""
-    global _torch
+    global _torch, _stream
     if _torch is None:
         import torch
         lib = _runtime.library()
@@ -64,6 +65,7 @@ def _load():
             raise RuntimeError('two HIP runtimes are loaded (' + ', '.join(sorted(loaded)) +
                                '): import torch before the first call into the library')
         _types.update({torch.float32: _F32, torch.float16: _F16, torch.bfloat16: _BF16})
+        _stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
         _torch = torch
         return torch, lib
     return _torch, _runtime._lib
@@ -72,6 +74,11 @@ def _load():
 def _need(ok, message):
     if not ok:
         raise ValueError(message)
+
+
+def _sig(t):
+    """All that the checks ask of a tensor argument but its address."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
 
 
 class KvCache:
@@ -156,7 +163,7 @@ class KvCache:
                               keys.data_ptr(), values.data_ptr(), key_params.data_ptr() if int4 else None,
                               value_params.data_ptr() if int4 else None, positions.data_ptr())
         self._address = ctypes.addressof(self._struct)
-        self._workspaces = {}
+        self._plans = {}  # checked argument structs by the arguments' shapes, strides and types
 
     @staticmethod
     def _row_strides(t, row):
@@ -227,16 +234,61 @@ class KvCache:
         return (s[0] if len(shape) == 4 and shape[0] > 1 else s[-3]), s[-2]
 
 
+    def _plan(self, key, make):
+        """The checked structs of a call; the same shapes, strides and types are checked once."""
+        plan = self._plans.get(key)
+        if plan is None:
+            plan = make()
+            if len(self._plans) >= 256:
+                self._plans.clear()
+            self._plans[key] = plan
+        return plan
+
+
 def _launch(device, call, *args):
-    torch, _ = _load()
-    if torch.cuda.current_device() == device.index:
-        status = call(*args, torch.cuda.current_stream(device).cuda_stream)
+    torch = _torch
+    index = device.index
+    if torch.cuda.current_device() == index:
+        status = call(*args, _stream(index))
     else:
         with torch.cuda.device(device):
-            status = call(*args, torch.cuda.current_stream(device).cuda_stream)
+            status = call(*args, _stream(index))
     if status:
         message = _runtime._lib.st_last_error().decode() or f'libstamd error {status}'
         raise (ValueError if status == 1 else RuntimeError)(message)
+
+
+def _plan_append(cache, q, k, v, q_gain, k_gain, inv_freq, rope, rope_dims, pairs, offsets, max_tokens, out):
+    torch = _torch
+    tokens, rows = cache._rows(q, offsets, max_tokens)
+    dtype = q.dtype
+    _need(dtype in _types, 'q must be float32, float16 or bfloat16')
+    heads = q.shape[-2]
+    args = _Append()
+    args.dtype, args.q_heads = _types[dtype], heads
+    args.q_strides = cache._heads(q, q, heads, 'q', dtype)
+    args.k_strides = cache._heads(k, q, cache.kv_heads, 'k', dtype)
+    args.v_strides = cache._heads(v, q, cache.kv_heads, 'v', dtype)
+    args.out_strides = cache._heads(out, q, heads, 'out', dtype)
+    _need(pairs in ('adjacent', 'halves'), "pairs must be 'adjacent' or 'halves'")
+    _need(inv_freq is None or rope is None, 'give inv_freq or rope, not both')
+    if inv_freq is not None:
+        _need(inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous()
+              and inv_freq.device == cache.device, 'inv_freq must be float64 [rope_dims / 2] on the cache\'s device')
+        half = inv_freq.shape[0]
+    elif rope is not None:
+        _need(rope.dtype == torch.float32 and rope.dim() == 3 and rope.shape[0] == tokens and rope.shape[2] == 2
+              and rope.is_contiguous() and rope.device == cache.device,
+              'rope must be float32 [rows, rope_dims / 2, 2] on the cache\'s device')
+        half = rope.shape[1]
+    else:
+        half = 0
+    _need(rope_dims is None or rope_dims == 2 * half, 'rope_dims must be twice the frequencies\' number')
+    args.rope_dims, args.rope_halves = 2 * half, int(pairs == 'halves')
+    for name, gain in (('q_gain', q_gain), ('k_gain', k_gain)):
+        _need(gain is None or (gain.dtype == torch.float32 and gain.shape == (cache.head_dim,) and gain.is_contiguous()
+                               and gain.device == cache.device), f'{name} must be float32 [head_dim] on the cache\'s device')
+    return tokens, rows, args
 
 
 def qk_norm_rope_append(cache, q, k, v, *, q_gain=None, k_gain=None, epsilon=1e-6, inv_freq=None, rope=None,
@@ -255,55 +307,32 @@ def qk_norm_rope_append(cache, q, k, v, *, q_gain=None, k_gain=None, epsilon=1e-
     'halves' (i, i + rope_dims / 2)."""
     torch, lib = _load()
     _need(isinstance(cache, KvCache), 'cache must be a KvCache')
-    tokens, rows = cache._rows(q, offsets, max_tokens)
-    dtype = q.dtype
-    _need(dtype in _types, 'q must be float32, float16 or bfloat16')
-    heads = q.shape[-2]
-    args = _Append()
-    args.dtype, args.q_heads = _types[dtype], heads
-    for name, t, n in (('q', q, heads), ('k', k, cache.kv_heads), ('v', v, cache.kv_heads)):
-        setattr(args, name + '_strides', cache._heads(t, q, n, name, dtype))
-        setattr(args, name, t.data_ptr())
-    _need(pairs in ('adjacent', 'halves'), "pairs must be 'adjacent' or 'halves'")
-    _need(inv_freq is None or rope is None, 'give inv_freq or rope, not both')
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    key = (_sig(q), _sig(k), _sig(v), _sig(q_gain), _sig(k_gain), _sig(inv_freq), _sig(rope), rope_dims, pairs, _sig(offsets),
+           max_tokens, _sig(out))
+    tokens, rows, args = cache._plan(key, lambda: _plan_append(cache, q, k, v, q_gain, k_gain, inv_freq, rope, rope_dims, pairs,
+                                                               offsets, max_tokens, out))
+    if not tokens:
+        return out
+    args = _Append.from_buffer_copy(args)
+    args.q, args.k, args.v, args.q_out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    if q_gain is not None:
+        args.q_gain = q_gain.data_ptr()
+    if k_gain is not None:
+        args.k_gain = k_gain.data_ptr()
+    args.epsilon = epsilon
     if inv_freq is not None:
-        _need(inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous()
-              and inv_freq.device == cache.device, 'inv_freq must be float64 [rope_dims / 2] on the cache\'s device')
-        half = inv_freq.shape[0]
         args.inv_freq = inv_freq.data_ptr()
     elif rope is not None:
-        _need(rope.dtype == torch.float32 and rope.dim() == 3 and rope.shape[0] == tokens and rope.shape[2] == 2
-              and rope.is_contiguous() and rope.device == cache.device,
-              'rope must be float32 [rows, rope_dims / 2, 2] on the cache\'s device')
-        half = rope.shape[1]
         args.rope = rope.data_ptr()
-    else:
-        half = 0
-    _need(rope_dims is None or rope_dims == 2 * half, 'rope_dims must be twice the frequencies\' number')
-    args.rope_dims, args.rope_halves = 2 * half, int(pairs == 'halves')
-    for name, gain in (('q_gain', q_gain), ('k_gain', k_gain)):
-        if gain is not None:
-            _need(gain.dtype == torch.float32 and gain.shape == (cache.head_dim,) and gain.is_contiguous()
-                  and gain.device == cache.device, f'{name} must be float32 [head_dim] on the cache\'s device')
-            setattr(args, name, gain.data_ptr())
-    args.epsilon = epsilon
-    if out is None:
-        out = torch.empty(q.shape, dtype=dtype, device=cache.device)
-    args.out_strides = cache._heads(out, q, heads, 'out', dtype)
-    args.q_out = out.data_ptr()
-    if tokens:
-        _launch(cache.device, lib.st_qk_norm_rope_append, cache._address, ctypes.addressof(rows), ctypes.addressof(args))
+    if offsets is not None:
+        rows = _Rows(rows.tokens, rows.max_tokens, offsets.data_ptr())
+    _launch(cache.device, lib.st_qk_norm_rope_append, cache._address, ctypes.addressof(rows), ctypes.addressof(args))
     return out
 
 
-def window_attention(cache, q, *, scale=None, offsets=None, max_tokens=None, out=None):
-    """Attention of new tokens' queries over the cache, which holds their keys and values already
-    (:func:`qk_norm_rope_append`): each query sees the sinks and the last `window` positions up to its own.
-    q, offsets, max_tokens and out as there, and q_heads a multiple of the cache's heads: query head h reads
-    cache head h // (q_heads // kv_heads). scale: 1 / sqrt(head_dim) if None. Float32 queries go with every
-    cache, 16-bit ones with a cache of their own type or a 4-bit one."""
-    torch, lib = _load()
-    _need(isinstance(cache, KvCache), 'cache must be a KvCache')
+def _plan_attention(cache, q, offsets, max_tokens, out):
     tokens, rows = cache._rows(q, offsets, max_tokens)
     dtype = q.dtype
     _need(dtype in _types, 'q must be float32, float16 or bfloat16')
@@ -311,23 +340,36 @@ def window_attention(cache, q, *, scale=None, offsets=None, max_tokens=None, out
     args = _Attention()
     args.dtype, args.q_heads = _types[dtype], heads
     args.q_strides = cache._heads(q, q, heads, 'q', dtype)
-    args.q = q.data_ptr()
-    if out is None:
-        out = torch.empty(q.shape, dtype=dtype, device=cache.device)
     args.out_strides = cache._heads(out, q, heads, 'out', dtype)
-    args.out = out.data_ptr()
-    args.scale = 1.0 / math.sqrt(cache.head_dim) if scale is None else scale
+    if tokens:
+        size = ctypes.c_size_t(0)
+        _launch(cache.device, lambda *a: _runtime._lib.st_window_attention_workspace(*a[:-1]), cache._address,
+                ctypes.addressof(rows), heads, _types[dtype], ctypes.byref(size))
+        args.workspace_bytes = size.value
+    return tokens, rows, args
+
+
+def window_attention(cache, q, *, scale=None, offsets=None, max_tokens=None, out=None):
+    """Attention of new tokens' queries over the cache, which holds their keys and values already
+    (:func:`qk_norm_rope_append`): each query sees the sinks and the last `window` positions up to its own.
+    q, offsets, max_tokens and out as there, and q_heads a multiple of the cache's heads: query head h reads
+    cache head h // (q_heads // kv_heads). scale: 1 / sqrt(head_dim) if None, positive. Float32 queries go with
+    every cache, 16-bit ones with a cache of their own type or a 4-bit one."""
+    torch, lib = _load()
+    _need(isinstance(cache, KvCache), 'cache must be a KvCache')
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    key = (_sig(q), _sig(offsets), max_tokens, _sig(out))
+    tokens, rows, args = cache._plan(key, lambda: _plan_attention(cache, q, offsets, max_tokens, out))
     if not tokens:
         return out
-    key = (rows.max_tokens, heads, dtype)
-    need = cache._workspaces.get(key)
-    if need is None:
-        size = ctypes.c_size_t(0)
-        _launch(cache.device, lambda *a: lib.st_window_attention_workspace(*a[:-1]), cache._address, ctypes.addressof(rows),
-                heads, _types[dtype], ctypes.byref(size))
-        need = cache._workspaces[key] = size.value
-    if need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=cache.device)
-        args.workspace, args.workspace_bytes = workspace.data_ptr(), need
+    args = _Attention.from_buffer_copy(args)
+    args.q, args.out = q.data_ptr(), out.data_ptr()
+    args.scale = 1.0 / math.sqrt(cache.head_dim) if scale is None else scale
+    if args.workspace_bytes:
+        workspace = torch.empty(args.workspace_bytes, dtype=torch.uint8, device=cache.device)
+        args.workspace = workspace.data_ptr()
+    if offsets is not None:
+        rows = _Rows(rows.tokens, rows.max_tokens, offsets.data_ptr())
     _launch(cache.device, lib.st_window_attention, cache._address, ctypes.addressof(rows), ctypes.addressof(args))
     return out
