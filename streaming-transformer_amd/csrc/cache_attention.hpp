@@ -108,18 +108,22 @@ struct RowLoad {
   static constexpr int L = D / E;
 };
 
-// The 32 codes of a 4-bit load and their (scale, minimum) as 16-bit or FP32 values. FP16: code + 1024 (or
-// + 64 for the codes in bits 4 and 12 of a half) is made by an OR, the constant subtracted exactly, and
-// minimum + scale * code is rounded once, to FP16 (2^-12 of the value, for 16-bit queries only).
-__device__ __forceinline__ word4_t dequant8_f16(unsigned w, half2_t s, half2_t z) {
+// Eight codes of a 4-bit row and their (scale, minimum) as FP16 values. code + 1024 (or + 64 for the codes in
+// bits 4 and 12 of a half) is made by an OR, the constant subtracted exactly. term 0: minimum + scale * code
+// rounded once, to FP16; term 1: what that rounding left, from the FP32 value.
+template <int kTerm>
+__device__ __forceinline__ word4_t dequant8_f16(unsigned w, half2_t sz) {
   const half2_t big = {(_Float16)1024.f, (_Float16)1024.f}, mid = {(_Float16)64.f, (_Float16)64.f};
-  auto a = [&](unsigned x) {
-    return __builtin_bit_cast(unsigned, (__builtin_bit_cast(half2_t, (x & 0x000f000fu) | 0x64006400u) - big) * s + z);
+  const half2_t s = {sz[0], sz[0]}, z = {sz[1], sz[1]};
+  auto value = [&](half2_t code) {
+    const half2_t v = code * s + z;
+    if constexpr (kTerm == 0) return __builtin_bit_cast(unsigned, v);
+    const float a = (float)code[0] * (float)sz[0] + (float)sz[1], b = (float)code[1] * (float)sz[0] + (float)sz[1];
+    return pack_f16(a - (float)v[0], b - (float)v[1]);
   };
-  auto b = [&](unsigned x) {
-    return __builtin_bit_cast(unsigned, (__builtin_bit_cast(half2_t, (x & 0x00f000f0u) | 0x54005400u) - mid) * s + z);
-  };
-  return word4_t{a(w), b(w), a(w >> 8), b(w >> 8)};
+  auto low = [&](unsigned x) { return value(__builtin_bit_cast(half2_t, (x & 0x000f000fu) | 0x64006400u) - big); };
+  auto high = [&](unsigned x) { return value(__builtin_bit_cast(half2_t, (x & 0x00f000f0u) | 0x54005400u) - mid); };
+  return word4_t{low(w), high(w), low(w >> 8), high(w >> 8)};
 }
 __device__ __forceinline__ void dequant8_f32(unsigned w, float s, float z, float4_t (&out)[2]) {
 #pragma unroll
@@ -130,8 +134,8 @@ __device__ __forceinline__ void dequant8_f32(unsigned w, float s, float z, float
 }
 
 // One 16-byte load of row r, lane position p of the row's L, as the chunks of the LDS tile: calls
-// put(chunk, value) for each. `keep`: whether the lane's elements are inside the head.
-template <int C, int M, typename Put>
+// put(chunk, value) for each. `keep`: whether the lane's elements are inside the head. kTerm: of 4-bit rows.
+template <int C, int M, int kTerm = 0, typename Put>
 __device__ __forceinline__ void expand(word4_t w, unsigned params, int p, bool keep, Put&& put) {
   if (!keep) {
     w = word4_t{0, 0, 0, 0};
@@ -151,7 +155,7 @@ __device__ __forceinline__ void expand(word4_t w, unsigned params, int p, bool k
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; i++) put(p * 4 + i, dequant8_f16(w[i], half2_t{sz[0], sz[0]}, half2_t{sz[1], sz[1]}));
+      for (int i = 0; i < 4; i++) put(p * 4 + i, dequant8_f16<kTerm>(w[i], sz));
     }
   } else {
     static_assert(M == kTF32);
@@ -214,6 +218,14 @@ __device__ __forceinline__ void load_to_lds(const char* from, char* to) {
 }
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
+// FP16 queries over 4-bit rows: the rounding of the dequantised values to FP16 is as large as the output's own,
+// twice (K and V), and the weights' a third. Keys in two FP16 terms and weights in two leave one of the three
+// (the output of 4 x 1024 tokens 1.9 times as far from exact as its own rounding without, 1.35 with).
+template <int A, int C>
+constexpr bool two_terms() {
+  return A == kTF16 && C == kTInt4;
+}
+
 // The type that the MFMAs take: FP32 for FP32 queries (every cache type widens to it exactly), else the
 // queries' own; 4-bit rows become FP16 for bfloat16 queries too, whose eight significant bits FP16 holds
 // once the row is scaled by a power of two.
@@ -269,12 +281,15 @@ struct QueryBlock {
 };
 
 // Products of one tile with a block of 16 rows, for a wave. kt and vt: the tile's K and V in LDS.
-template <int M, int D, int KT>
+// kFine: 16-bit weights in two terms (w and what its rounding left), so that the output's own rounding is
+// the only one that counts; twice the products with V.
+template <int M, int D, int KT, bool kFine>
 struct TileMath {
   using T = TileLayout<M, D>;
   static constexpr int kBlocks = KT / 16;
   // S^T of the tile for MB blocks of rows. Each depth's products go over all blocks: independent sums.
-  template <int MB, typename Q>
+  // kMore: added to what s holds.
+  template <bool kMore, int MB, typename Q>
   __device__ static __forceinline__ void logits(const char* kt, const Q (&q)[MB], float4_t (&s)[MB][kBlocks], int lane) {
     const int g = lane >> 4;
 #pragma unroll
@@ -285,7 +300,7 @@ struct TileMath {
         const word4_t k = lds_load<word4_t>(kt + r * T::kRow + T::key_chunk(r, step * 4 + g) * 16);
 #pragma unroll
         for (int u = 0; u < MB; u++)
-          s[u][kb] = Mfma<M>::mul(k, q[u].f[step], step == 0 ? float4_t{0.f, 0.f, 0.f, 0.f} : s[u][kb]);
+          s[u][kb] = Mfma<M>::mul(k, q[u].f[step], step == 0 && !kMore ? float4_t{0.f, 0.f, 0.f, 0.f} : s[u][kb]);
       }
     }
     // Six reads ahead of the products, then one per MB of them: left alone, the compiler waits for most reads
@@ -383,7 +398,7 @@ struct TileMath {
                                                  const float (&base)[MB], float4_t (&o)[MB][D / 16 + 1], int lane) {
 #pragma unroll
     for (int depth = 0; depth < kDepths; depth++) {
-      word4_t w[MB];
+      word4_t w[MB], rest[MB];
 #pragma unroll
       for (int u = 0; u < MB; u++) {
         float p[kDepth / 4];
@@ -396,8 +411,14 @@ struct TileMath {
           o[u][D / 16] += x;
         } else {
           constexpr unsigned one = M == kTF16 ? 0x3c003c00u : 0x3f803f80u;
-          w[u] = word4_t{pack16<M>(p[0], p[1]), pack16<M>(p[2], p[3]), pack16<M>(p[4], p[5]), pack16<M>(p[6], p[7])};
-          o[u][D / 16] = Mfma<M>::mul(word4_t{one, one, one, one}, w[u], o[u][D / 16]);
+          const word4_t ones = {one, one, one, one};
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            w[u][i] = pack16<M>(p[2 * i], p[2 * i + 1]);
+            if constexpr (kFine) rest[u][i] = pack16<M>(p[2 * i] - low16<M>(w[u][i]), p[2 * i + 1] - high16<M>(w[u][i]));
+          }
+          o[u][D / 16] = Mfma<M>::mul(ones, w[u], o[u][D / 16]);
+          if constexpr (kFine) o[u][D / 16] = Mfma<M>::mul(ones, rest[u], o[u][D / 16]);
         }
       }
 #pragma unroll
@@ -405,6 +426,10 @@ struct TileMath {
         const word4_t v = values(vt, depth, d, lane);
 #pragma unroll
         for (int u = 0; u < MB; u++) o[u][d] = Mfma<M>::mul(v, w[u], o[u][d]);
+        if constexpr (kFine) {
+#pragma unroll
+          for (int u = 0; u < MB; u++) o[u][d] = Mfma<M>::mul(v, rest[u], o[u][d]);
+        }
       }
     }
   }
@@ -519,7 +544,8 @@ __global__ __launch_bounds__(64 * kWaves, 2 * 4 / kWaves) void cache_attention(C
   constexpr int KT = wave_tile<M, D>();
   using T = TileLayout<M, D>;
   using R = RowLoad<C, D>;
-  using X = TileMath<M, D, KT>;
+  // (FP16 weights are far finer than a bfloat16 output.)
+  using X = TileMath<M, D, KT, M != kTF32 && M == A>;
   constexpr int kPerLoad = 64 / R::L;                                // rows of one load of the wave
   constexpr int kLoads = (KT + kPerLoad - 1) / kPerLoad;
   static_assert(KT % kPerLoad == 0);
@@ -626,11 +652,20 @@ __global__ __launch_bounds__(64 * kWaves, 2 * 4 / kWaves) void cache_attention(C
       X::template clear<64>(vt, lane);
       wave_sync();
     }
-    load(min(tile + kWaves, t1 - 1) * KT);
-
     float4_t s[MB][X::kBlocks];
     float base[MB];
-    X::logits(kt, q, s, lane);
+    if constexpr (two_terms<A, C>()) {
+      X::template logits<false>(kt, q, s, lane);
+      wave_sync();
+#pragma unroll
+      for (int i = 0; i < kLoads; i++) {
+        const int row = i * kPerLoad + sub;
+        expand<C, M, 1>(kw[i], kp[i], p, keep, [&](int ch, word4_t w) { lds_put(kt + row * T::kRow + T::key_chunk(row, ch) * 16, w); });
+      }
+      wave_sync();
+    }
+    load(min(tile + kWaves, t1 - 1) * KT);
+    X::template logits<two_terms<A, C>()>(kt, q, s, lane);
     if (!whole) X::mask(s, seen, keys, c.window, j0, lane);
     move_maxima(s, q, m, base, o);
     X::outputs(vt, s, q, base, o, lane);
@@ -914,29 +949,37 @@ __global__ __launch_bounds__(64 * kVectorWaves) void cache_attention_vector(Cach
 }
 
 // Many rows (prompts, long pieces): bound by the matrix products. Workgroup (kv head, row tile; stream):
-// four waves of MB blocks of 16 rows each. The tile of keys is the workgroup's, staged once for its rows:
+// waves of MB blocks of 16 rows each. The tile of keys is the workgroup's, staged once for its rows:
 // two tiles of LDS, so that one is computed while the next one's loads are in flight (straight to LDS where the
 // rows need no conversion), and one barrier per tile. Row tiles of one (stream, kv head) follow each other in the grid at steps of
 // kv_heads, those that see most keys first: with eight heads, or a multiple, each XCD's L2 holds one head's keys.
-constexpr int kRowsThreads = 256;
 template <int M, int D>
 constexpr int rows_tile() {
   return M == kTF32 ? 4096 / D : D == 256 ? 32 : 64;
 }
+// Waves of a workgroup: eight where rows are converted on their way (which costs the less per row the more rows
+// share it; half of the threads take K, half V), else four, two workgroups per CU. Head dimension 256 leaves
+// registers for four waves on a CU.
+constexpr int rows_waves(int type, int stored, int dim) { return type == stored || dim > 128 ? 4 : 8; }
+constexpr int rows_threads(int type, int stored, int dim) { return 64 * rows_waves(type, stored, dim); }
+constexpr int rows_per_cu(int type, int stored, int dim) { return dim > 128 ? 1 : 8 / rows_waves(type, stored, dim); }
 template <int A, int C, int D, int MB>
-__global__ __launch_bounds__(kRowsThreads, D == 256 ? 1 : 2) void cache_attention_rows(CacheView c, RowsView r, AttentionView a) {
+__global__ __launch_bounds__(rows_threads(A, C, D), rows_per_cu(A, C, D))
+void cache_attention_rows(CacheView c, RowsView r, AttentionView a) {
   constexpr int M = mfma_type<A, C>();
   constexpr int KT = rows_tile<M, D>();
   using T = TileLayout<M, D>;
   using R = RowLoad<C, D>;
-  using X = TileMath<M, D, KT>;
-  constexpr int kWaves = kRowsThreads / 64, kRows = kWaves * MB * 16;
-  constexpr int kPerLoad = kRowsThreads / R::L;  // rows of one load of the workgroup
+  constexpr bool kTwo = two_terms<A, C>();  // both terms of K are staged
+  using X = TileMath<M, D, KT, kTwo>;
+  constexpr bool kDirect = C == M;
+  constexpr int kWaves = rows_waves(A, C, D), kThreads = 64 * kWaves, kRows = kWaves * MB * 16;
+  constexpr int kLoaders = kDirect ? kThreads : kThreads / 2;  // of one of K and V
+  constexpr int kPerLoad = kLoaders / R::L;  // rows of one load of theirs
   constexpr int kLoads = (KT + kPerLoad - 1) / kPerLoad;
   constexpr int kTile = KT * T::kRow;
-  constexpr bool kDirect = C == M;
   static_assert(!kDirect || KT % kPerLoad == 0);
-  __shared__ __attribute__((aligned(16))) char lds[2][2][kTile];
+  __shared__ __attribute__((aligned(16))) char lds[2][kTwo ? 3 : 2][kTile];
 
   const int head = blockIdx.x % c.kv_heads, b = blockIdx.y;
   const int64_t start = uniform64(c.positions[b]);
@@ -951,7 +994,8 @@ __global__ __launch_bounds__(kRowsThreads, D == 256 ? 1 : 2) void cache_attentio
   KeyList keys;
   keys.init(c, start + row0 / a.group, start + last_row / a.group);
 
-  const int p = threadIdx.x % R::L, sub = threadIdx.x / R::L;
+  const int loader = threadIdx.x % kLoaders, p = loader % R::L, sub = loader / R::L;
+  const bool is_v = threadIdx.x >= kLoaders;  // of those that load to registers
   const bool keep = p * R::E < c.dim;
   const int64_t base_row = b * c.stream_stride + head * c.head_stride;
   const char* kbase = c.keys + base_row * c.row_bytes;
@@ -960,8 +1004,10 @@ __global__ __launch_bounds__(kRowsThreads, D == 256 ? 1 : 2) void cache_attentio
   const char* vpbase = C == kTInt4 ? reinterpret_cast<const char*>(c.value_params) + base_row * (c.row_bytes / 4) : nullptr;
   const uint32_t slot_bytes = c.slot_stride * c.row_bytes, chunk = keep ? p * 16 : 0, pair = keep ? p : 0;
   const bool near = slot_bytes < 1u << 25;  // a tile's rows within 32 bits of its first
-  word4_t kw[kLoads], vw[kLoads];
-  unsigned kp[kLoads], vp[kLoads];
+  word4_t raw[kLoads];
+  unsigned params[kLoads];
+  const char* const base = is_v ? vbase : kbase;
+  const char* const pbase = is_v ? vpbase : kpbase;
   const uint32_t part = min(sub, KT - 1) * slot_bytes;
   const int wave = wave_id(), lane = lane_id(), g = lane >> 4;
   // The loads of the tile at entry j0: rows that need no conversion go straight to LDS, others to registers.
@@ -972,7 +1018,7 @@ __global__ __launch_bounds__(kRowsThreads, D == 256 ? 1 : 2) void cache_attentio
       // A wave's load fills 64 consecutive chunks of the tile: the lane fetches the one that belongs there.
 #pragma unroll
       for (int i = 0; i < kLoads; i++) {
-        const int row = i * kPerLoad + sub, to = (i * kRowsThreads + wave * 64) * 16;
+        const int row = i * kPerLoad + sub, to = (i * kThreads + wave * 64) * 16;
         const int kc = T::key_chunk(row, p), vc = T::value_chunk(row, p);
         if (kc * R::E < c.dim) load_to_lds(kbase + at[i] + kc * 16, lds[buffer][0] + to);
         if (vc * R::E < c.dim) load_to_lds(vbase + at[i] + vc * 16, lds[buffer][1] + to);
@@ -980,13 +1026,8 @@ __global__ __launch_bounds__(kRowsThreads, D == 256 ? 1 : 2) void cache_attentio
     } else {
 #pragma unroll
       for (int i = 0; i < kLoads; i++) {
-        kw[i] = load_global<word4_t>(kbase + at[i] + chunk);
-        vw[i] = load_global<word4_t>(vbase + at[i] + chunk);
-        if constexpr (C == kTInt4) {
-          const uint64_t params = at[i] / 16 * 4 + pair * 4;  // 16 bytes of codes have 4 of scale and minimum
-          kp[i] = load_global<unsigned>(kpbase + params);
-          vp[i] = load_global<unsigned>(vpbase + params);
-        }
+        raw[i] = load_global<word4_t>(base + at[i] + chunk);
+        if constexpr (C == kTInt4) params[i] = load_global<unsigned>(pbase + at[i] / 16 * 4 + pair * 4);  // 4 bytes of 16
       }
     }
   };
@@ -998,24 +1039,29 @@ __global__ __launch_bounds__(kRowsThreads, D == 256 ? 1 : 2) void cache_attentio
       if (look) {
 #pragma unroll
         for (int i = 0; i < kLoads; i++)
-          found |= not_finite<M>(lds_load<word4_t>(lds[buffer][1] + (i * kRowsThreads + (int)threadIdx.x) * 16));
+          found |= not_finite<M>(lds_load<word4_t>(lds[buffer][1] + (i * kThreads + (int)threadIdx.x) * 16));
       }
     } else {
 #pragma unroll
       for (int i = 0; i < kLoads; i++) {
         const int row = i * kPerLoad + sub;
         if (KT % kPerLoad != 0 && row >= KT) break;
-        expand<C, M>(kw[i], kp[i], p, keep, [&](int ch, word4_t w) { lds_put(lds[buffer][0] + row * T::kRow + T::key_chunk(row, ch) * 16, w); });
-        expand<C, M>(vw[i], vp[i], p, keep, [&](int ch, word4_t w) {
-          lds_put(lds[buffer][1] + row * T::kRow + T::value_chunk(row, ch) * 16, w);
-          if (look) found |= not_finite<M>(w);
-        });
+        if (!is_v) {
+          expand<C, M>(raw[i], params[i], p, keep, [&](int ch, word4_t w) { lds_put(lds[buffer][0] + row * T::kRow + T::key_chunk(row, ch) * 16, w); });
+          if constexpr (kTwo)
+            expand<C, M, 1>(raw[i], params[i], p, keep, [&](int ch, word4_t w) { lds_put(lds[buffer][2] + row * T::kRow + T::key_chunk(row, ch) * 16, w); });
+        } else {
+          expand<C, M>(raw[i], params[i], p, keep, [&](int ch, word4_t w) {
+            lds_put(lds[buffer][1] + row * T::kRow + T::value_chunk(row, ch) * 16, w);
+            if (look) found |= not_finite<M>(w);
+          });
+        }
       }
     }
     return found;
   };
   if (kDirect && c.dim < D) {  // the padding, which no load writes
-    for (int at = threadIdx.x * 16; at < 4 * kTile; at += kRowsThreads * 16) lds_put(&lds[0][0][0] + at, word4_t{0, 0, 0, 0});
+    for (int at = threadIdx.x * 16; at < (int)sizeof(lds); at += kThreads * 16) lds_put(&lds[0][0][0] + at, word4_t{0, 0, 0, 0});
     __syncthreads();
   }
 
@@ -1051,7 +1097,7 @@ __global__ __launch_bounds__(kRowsThreads, D == 256 ? 1 : 2) void cache_attentio
 
   // One tile. kWhole: all of the workgroup's rows see all of it.
   auto step = [&](int tile, auto kWhole) {
-    const int j0 = tile * KT, buffer = tile & 1;
+    const int j0 = tile * KT, buffer = tile & 1, other = buffer ^ 1;
     const char* kt = lds[buffer][0];
     char* vt = lds[buffer][1];
     bool none = false;
@@ -1060,24 +1106,27 @@ __global__ __launch_bounds__(kRowsThreads, D == 256 ? 1 : 2) void cache_attentio
       if (odd) {
         if (!none) X::add_odd(vt, o, lane, [&](int u, int e) { return seen[u](keys, c.window, j0 + e); });
         __syncthreads();
-        X::template clear<kRowsThreads>(vt, threadIdx.x);
+        X::template clear<kThreads>(vt, threadIdx.x);
         __syncthreads();
       }
     }
     float4_t s[MB][X::kBlocks];
     float base[MB];
-    if (!none) X::logits(kt, q, s, lane);
+    if (!none) {
+      X::template logits<false>(kt, q, s, lane);
+      if constexpr (kTwo) X::template logits<true>(lds[buffer][2], q, s, lane);
+    }
     // The next tile's loads, after the reads of K: the compiler lets no LDS read pass a load to LDS before it has
     // arrived, and the next ones are V's, behind the maxima. Loads to registers have no condition around them, and
     // repeat the last tile: with one, or in two forms, the compiler moves what they return and waits for it.
-    if (!kDirect || tile + 1 < tiles) load(min(tile + 1, tiles - 1) * KT, buffer ^ 1);
+    if (!kDirect || tile + 1 < tiles) load(min(tile + 1, tiles - 1) * KT, other);
     if (!none) {
       if constexpr (!kWhole) X::mask(s, seen, keys, c.window, j0, lane);
       move_maxima(s, q, m, base, o);
       X::outputs(vt, s, q, base, o, lane);
     }
     if (tile + 1 < tiles) {
-      const bool look = partial(j0 + KT), found = stage(buffer ^ 1, look);
+      const bool look = partial(j0 + KT), found = stage(other, look);
       if (look) odd = __syncthreads_or(found) != 0;
       else {
         odd = false;

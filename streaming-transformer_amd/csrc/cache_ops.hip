@@ -76,7 +76,8 @@ Plan plan_attention(const CacheView& c, const RowsView& r, int q_heads, int dtyp
   if (rows > 64) {
     p.many = true;
     p.blocks = padded == 256 ? 1 : 2;
-    p.tiles = (rows + 64 * p.blocks - 1) / (64 * p.blocks);
+    const int tile = 16 * p.blocks * rows_waves(dtype, stored, padded);
+    p.tiles = (rows + tile - 1) / tile;
     p.splits = 1;
     return p;
   }
@@ -113,7 +114,7 @@ void launch_attention(const CacheView& c, const RowsView& r, const AttentionView
   auto go = [&](auto kernel, int threads) { hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, stream, c, r, a); };
   auto form = [&](auto D) {
     constexpr int d = decltype(D)::value;
-    if (p.many) return go(cache_attention_rows<A, C, d, d == 256 ? 1 : 2>, kRowsThreads);
+    if (p.many) return go(cache_attention_rows<A, C, d, d == 256 ? 1 : 2>, rows_threads(A, C, d));
     if constexpr (A == kTF32) {
       if (p.vector == 1) return go(cache_attention_vector<C, d, 1>, 64 * kVectorWaves);
       if (p.vector == 2) return go(cache_attention_vector<C, d, 2>, 64 * kVectorWaves);
