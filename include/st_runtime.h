@@ -225,6 +225,9 @@ int st_transport_bench(const char* mode, uint64_t count, int32_t backoff, const 
 /* Json probe() - src/cuda/Runtime.cu:134-161, as a JSON string. */
 int st_probe_json(char* buffer, size_t cap, size_t* needed);
 
+/* Element types of the cache operators and of a batch's K/V. INT4 is storage only. */
+enum { ST_TYPE_F32 = 0, ST_TYPE_F16 = 1, ST_TYPE_BF16 = 2, ST_TYPE_INT4 = 3 };
+
 /* Extension (no counterpart in the reference, which is single-stream by design,
  * docs/Architecture.md:3): `streams` independent streams (1..256) sharing one set of
  * weights, each with its own K/V ring, hidden state and position. FP32 checkpoints with FP32
@@ -234,6 +237,27 @@ int st_probe_json(char* buffer, size_t cap, size_t* needed);
 typedef struct st_batch st_batch;
 int st_batch_create(const st_config* config, int32_t mixed, const st_tensor* tensors, size_t tensor_count,
                     int32_t streams, int32_t weight_dtype, st_batch** out);
+/* The same batch with more choices, for FP32 checkpoints (st_batch_create's are the default
+ * options, and give the same batch):
+ *   sinks      the first events of each stream, up to 4096, that stay visible beside the window;
+ *   head_norm  1: an RMS norm of each query and key head before its rotation, with the model's
+ *              epsilon and the gains "layers.{l}.q_norm" and ".k_norm" [head dim] among the tensors;
+ *   kv_dtype   the type that K and V are kept in (ST_TYPE_*); ST_KV_AS_MODEL: FP32, or a mixed
+ *              checkpoint's FP16.
+ * Any of them runs the steps' K/V through the cache operators below (head dimension a multiple of
+ * 8 up to 256; INT4 of 32). st_batch_snapshot then writes keys and values as
+ * [layer][head][sinks + window slots][dim], what the stored rows stand for. A stream's results
+ * depend on the batch around it only by the order of its attention's sums. */
+enum { ST_KV_AS_MODEL = -1 };
+typedef struct {
+  int32_t weight_dtype; /* as in st_options */
+  int32_t sinks;
+  int32_t head_norm;
+  int32_t kv_dtype;
+} st_batch_options;
+void st_batch_options_default(st_batch_options* options);
+int st_batch_create_with(const st_config* config, int32_t mixed, const st_tensor* tensors, size_t tensor_count,
+                         int32_t streams, const st_batch_options* options, st_batch** out);
 /* Extension, the same batch as one resident launch per step: stream s runs the fused
  * single-stream step on its own share of the CUs (workgroups [s*per, (s+1)*per), per = the
  * CU count / streams, a multiple of 8 when at least 8), with its own state and the weights
@@ -271,9 +295,6 @@ int st_batch_set_eager(st_batch* batch, int32_t eager);
  * allocate or copy, so they can be captured into a graph. All pointers inside the argument
  * structs are device memory. Calls on one cache run in the order of their streams; calls whose
  * work may overlap need caches, outputs and workspaces of their own. */
-
-/* Element types. INT4 is a cache's storage only. */
-enum { ST_TYPE_F32 = 0, ST_TYPE_F16 = 1, ST_TYPE_BF16 = 2, ST_TYPE_INT4 = 3 };
 
 /* A cache of keys and values with a sliding window and sinks (first positions that stay
  * visible). For each stream and head it has sinks + ring rows (slots): position p lives in slot p

@@ -16,8 +16,9 @@
 namespace stamd {
 
 Batch::Batch(const st_config& config, bool mixed, const st_tensor* tensors, size_t count, int streams,
-             int weight_dtype)
-    : c_(config) {
+             const st_batch_options& options)
+    : c_(config), options_(options) {
+  const int weight_dtype = options.weight_dtype;
   validate_config(c_);
   if (streams < 1 || streams > kBatchMax)
     throw Error(ST_ERR_INVALID, "Streams must be between 1 and " + std::to_string(kBatchMax));
@@ -34,6 +35,15 @@ Batch::Batch(const st_config& config, bool mixed, const st_tensor* tensors, size
   streams_p_ = streams <= 16 ? 16 : streams <= 32 ? 32 : (streams + 63) / 64 * 64;
   dim_ = c_.width / c_.heads;
   if (dim_ % 4) throw Error(ST_ERR_INVALID, "Batched streams need a head dimension that is a multiple of 4");
+  if (options.kv_dtype < ST_KV_AS_MODEL || options.kv_dtype > ST_TYPE_INT4) throw Error(ST_ERR_INVALID, "Unknown K/V storage");
+  if (options.sinks < 0 || options.sinks > 4096) throw Error(ST_ERR_INVALID, "Sinks must be between 0 and 4096");
+  if (options.head_norm != 0 && options.head_norm != 1) throw Error(ST_ERR_INVALID, "head_norm must be 0 or 1");
+  kv_type_ = options.kv_dtype == ST_KV_AS_MODEL ? ST_TYPE_F32 : options.kv_dtype;
+  cached_ = options.sinks || options.head_norm || kv_type_ != ST_TYPE_F32 || (mixed && options.kv_dtype != ST_KV_AS_MODEL);
+  slots_ = c_.window + options.sinks;
+  if (cached_ && mixed) throw Error(ST_ERR_INVALID, "Sinks, head norms and K/V types are for FP32 checkpoints");
+  if (cached_ && (dim_ % 8 || dim_ > 256)) throw Error(ST_ERR_INVALID, "Sinks, head norms and K/V types need a head dimension that is a multiple of 8 up to 256");
+  if (kv_type_ == ST_TYPE_INT4 && dim_ % 32) throw Error(ST_ERR_INVALID, "4-bit K/V need a head dimension that is a multiple of 32");
   int device = 0;
   HIP_CHECK(hipGetDevice(&device));
   hipDeviceProp_t prop;
@@ -81,8 +91,9 @@ Batch::Batch(const st_config& config, bool mixed, const st_tensor* tensors, size
     HIP_CHECK(hipMemset(buf.ptr, 0, std::max<size_t>(floats * 4, 256)));
     return reinterpret_cast<float*>(buf.ptr);
   };
-  // K/V rings [L][B][H][W][dh]: FP32, or FP16 in mixed mode.
+  // K/V rings [L][B][H][W][dh]: FP32, or FP16 in mixed mode; the cache operators' [L][B][H][sinks + W][dh].
   block_words_ = (size_t)c_.width * c_.window * (prec_ == kMixed ? 2 : 4) / 4;
+  if (cached_) block_words_ = (size_t)c_.width * slots_ * (kv_type_ == ST_TYPE_F32 ? 8 : kv_type_ == ST_TYPE_INT4 ? 1 : 4) / 8;
   a.keys = zeroed(keys_, (size_t)c_.layers * streams_ * block_words_);
   a.values = zeroed(values_, (size_t)c_.layers * streams_ * block_words_);
   a.hidden = zeroed(hidden_, (size_t)streams_ * c_.layers * c_.width);
@@ -97,7 +108,7 @@ Batch::Batch(const st_config& config, bool mixed, const st_tensor* tensors, size
   a.q = zeroed(q_, (size_t)streams_p_ * a.width);
   host_out_.alloc((size_t)streams_ * 4);
   a.score = reinterpret_cast<float*>(host_out_.dev);
-  if (attn_split()) {
+  if (!cached_ && attn_split()) {
     const int row = 64 * (dim_ > 64 ? 2 : 1) + 2;
     attn_part_.alloc((size_t)streams_ * c_.heads * attn_chunks() * row * 4);
     zeroed(attn_count_, (size_t)streams_ * c_.heads);
@@ -105,6 +116,8 @@ Batch::Batch(const st_config& config, bool mixed, const st_tensor* tensors, size
   a.rope = reinterpret_cast<float2*>(zeroed(step_rope_, (size_t)streams_p_ * dim_));
   a.slot = reinterpret_cast<int*>(zeroed(step_slot_, (size_t)streams_p_));
   host_in_.alloc((size_t)streams_ * c_.features * 4);
+
+  if (cached_) build_cache(tensors, count);
 
   args_dev_.alloc(sizeof(BatchArgs));
   HIP_CHECK(hipMemcpy(args_dev_.ptr, &args_, sizeof(BatchArgs), hipMemcpyHostToDevice));
@@ -118,6 +131,93 @@ Batch::Batch(const st_config& config, bool mixed, const st_tensor* tensors, size
   launch();
   HIP_CHECK(hipStreamEndCapture(stream_, &graph_.g));
   graph_exec_.instantiate(graph_);
+}
+
+// The cache operators' arguments: one cache per layer, the rows of the QKV projection, the head norms' gains.
+void Batch::build_cache(const st_tensor* tensors, size_t count) {
+  auto zeroed = [](DeviceBuffer& buf, size_t bytes) {
+    buf.alloc(bytes);
+    HIP_CHECK(hipMemset(buf.ptr, 0, std::max<size_t>(bytes, 256)));
+  };
+  const int d = c_.width, heads = c_.heads;
+  zeroed(qkv_, (size_t)streams_p_ * 3 * d * 4);
+  if (kv_type_ == ST_TYPE_INT4) {
+    param_words_ = (size_t)heads * slots_ * (dim_ / 32);
+    zeroed(key_params_, (size_t)c_.layers * streams_ * param_words_ * 4);
+    zeroed(value_params_, (size_t)c_.layers * streams_ * param_words_ * 4);
+  }
+  for (int l = 0; l < c_.layers; l++) {
+    const size_t block = (size_t)l * streams_, offset = block * block_words_ * 4;
+    st_kv_cache k{};
+    k.streams = streams_;
+    k.kv_heads = heads;
+    k.head_dim = dim_;
+    k.window = k.ring = c_.window;
+    k.sinks = options_.sinks;
+    k.dtype = kv_type_;
+    k.keys = static_cast<char*>(keys_.ptr) + offset;
+    k.values = static_cast<char*>(values_.ptr) + offset;
+    if (param_words_) {
+      k.key_params = static_cast<uint32_t*>(key_params_.ptr) + block * param_words_;
+      k.value_params = static_cast<uint32_t*>(value_params_.ptr) + block * param_words_;
+    }
+    k.positions = static_cast<const int64_t*>(position_.ptr);
+    caches_.push_back(k);
+  }
+  if (options_.head_norm) {
+    std::vector<float> gains((size_t)c_.layers * 2 * dim_);
+    for (int l = 0; l < c_.layers; l++)
+      for (int i = 0; i < 2; i++) {
+        const std::string name = "layers." + std::to_string(l) + (i ? ".k_norm" : ".q_norm");
+        const st_tensor* found = nullptr;
+        for (size_t t = 0; t < count; t++)
+          if (name == tensors[t].name) found = &tensors[t];
+        if (!found) throw Error(ST_ERR_INVALID, "Missing tensor: " + name);
+        if (found->rank != 1 || found->shape[0] != dim_) throw Error(ST_ERR_INVALID, "Shape mismatch: " + name);
+        std::memcpy(&gains[((size_t)l * 2 + i) * dim_], found->data, (size_t)dim_ * 4);
+      }
+    gains_.alloc(gains.size() * 4);
+    HIP_CHECK(hipMemcpy(gains_.ptr, gains.data(), gains.size() * 4, hipMemcpyHostToDevice));
+  }
+  const float* rows = static_cast<const float*>(qkv_.ptr);
+  append_.dtype = attention_.dtype = ST_TYPE_F32;
+  append_.q_heads = attention_.q_heads = heads;
+  append_.q = rows;
+  append_.k = rows + d;
+  append_.v = rows + 2 * d;
+  append_.q_out = qkv_.ptr;  // the queries in place
+  for (int64_t* s : {append_.q_strides, append_.k_strides, append_.v_strides, append_.out_strides, attention_.q_strides,
+                     attention_.out_strides}) {
+    s[0] = 3 * d;
+    s[1] = dim_;
+  }
+  append_.epsilon = c_.epsilon;
+  append_.rope_dims = dim_;
+  append_.rope = reinterpret_cast<const float*>(args_.rope);  // of this step, for all layers
+  attention_.q = rows;
+  attention_.out = args_.attn;
+  attention_.scale = 1.f / std::sqrt((float)dim_);
+  const st_new_rows step{streams_, 1, nullptr};
+  const size_t bytes = attention_workspace(&caches_[0], &step, heads, ST_TYPE_F32);
+  if (bytes) {
+    workspace_.alloc(bytes);
+    attention_.workspace = workspace_.ptr;
+    attention_.workspace_bytes = bytes;
+  }
+}
+
+// Head norms, rotation, append and attention of one layer by the cache operators; the output goes to the
+// operand layout of the OUT projection.
+template <int P>
+void Batch::attend_cache(int layer) {
+  const st_new_rows step{streams_, 1, nullptr};
+  st_append_args a = append_;
+  if (options_.head_norm) {
+    a.q_gain = static_cast<const float*>(gains_.ptr) + (size_t)layer * 2 * dim_;
+    a.k_gain = a.q_gain + dim_;
+  }
+  append_rows(&caches_[layer], &step, &a, stream_);
+  attend_rows(&caches_[layer], &step, &attention_, stream_, P == kBf16w ? 2 : 1, args_.width_p);
 }
 
 Batch::~Batch() {
@@ -265,9 +365,17 @@ void Batch::launch_sequence() {
   project<P, kEpInput, false>(a.in, a.features_p, a.x, a.width_p, a.w_input, d, 0u, 0);
   for (int l = 0; l < c_.layers; l++) {
     const LayerWeights& w = a.layer[l];
-    normed(qkv, w, w.norm1, l, fold_qkv);
-    if (kv_nt) attend<P, true>(l);
-    else attend<P, false>(l);
+    if constexpr (P != kMixed) {
+      if (cached_) {
+        project<P, kEpQkvRows, true>(a.x, a.width_p, qkv_.ptr, 3 * d, w.qkv, 3 * d, w.norm1, l);
+        attend_cache<P>(l);
+      }
+    }
+    if (!cached_) {
+      normed(qkv, w, w.norm1, l, fold_qkv);
+      if (kv_nt) attend<P, true>(l);
+      else attend<P, false>(l);
+    }
     project<P, kEpOut, false>(a.attn, a.width_p, a.x, a.width_p, w.out, d, 0u, l);
     normed(gateup, w, w.norm2, l, fold_gateup);
     project<P, kEpDown, false>(a.act, a.ffn_p, a.x, a.width_p, w.down, d, 0u, l);
@@ -321,30 +429,55 @@ void Batch::reset(int stream) {
   if (stream < -1 || stream >= streams_) throw Error(ST_ERR_INVALID, "Stream index out of range");
   hipLaunchKernelGGL(batch_reset, dim3(256), dim3(256), 0, stream_, dargs_, stream, block_words_);
   HIP_CHECK(hipGetLastError());
+  if (param_words_)
+    for (const DeviceBuffer* p : {&key_params_, &value_params_}) {
+      hipLaunchKernelGGL(batch_clear, dim3(256), dim3(256), 0, stream_, static_cast<unsigned*>(p->ptr), c_.layers, streams_,
+                         stream, param_words_);
+      HIP_CHECK(hipGetLastError());
+    }
   sync();
 }
 
 void Batch::snapshot(int stream, uint64_t* position, float* keys, float* values, float* hidden) {
   if (stream < 0 || stream >= streams_) throw Error(ST_ERR_INVALID, "Stream index out of range");
   sync();
-  const size_t ring = (size_t)c_.layers * c_.width * c_.window;
+  const size_t ring = (size_t)c_.layers * c_.width * slots_;
   if (position)
     HIP_CHECK(hipMemcpy(position, args_.position + stream, 8, hipMemcpyDeviceToHost));
-  // The stream's block of each layer (layer-major rings) into [L][H][W][dh].
-  auto download = [&](const void* base, float* dst) {
+  // The stream's block of each layer (layer-major arrays), `words` 4-byte words each.
+  auto blocks = [&](void* dst, const void* base, size_t words) {
+    const size_t block = words * 4, pitch = (size_t)streams_ * block;
+    HIP_CHECK(hipMemcpy2D(dst, block, static_cast<const char*>(base) + (size_t)stream * block, pitch, block, c_.layers,
+                          hipMemcpyDeviceToHost));
+  };
+  // ... into [L][H][slots][dh] floats.
+  auto download = [&](const void* base, const DeviceBuffer& params, float* dst) {
     if (!dst) return;
-    const size_t block = block_words_ * 4, pitch = (size_t)streams_ * block;
-    const char* src = reinterpret_cast<const char*>(base) + (size_t)stream * block;
-    if (prec_ == kMixed) {
-      std::vector<uint16_t> h(ring);
-      HIP_CHECK(hipMemcpy2D(h.data(), block, src, pitch, block, c_.layers, hipMemcpyDeviceToHost));
-      for (size_t i = 0; i < ring; i++) dst[i] = host_half_to_float(h[i]);
-    } else {
-      HIP_CHECK(hipMemcpy2D(dst, block, src, pitch, block, c_.layers, hipMemcpyDeviceToHost));
+    const int type = prec_ == kMixed ? ST_TYPE_F16 : kv_type_;
+    if (type == ST_TYPE_F32) return blocks(dst, base, block_words_);
+    if (type == ST_TYPE_INT4) {
+      std::vector<uint32_t> codes(ring / 8), pairs(ring / 32);
+      blocks(codes.data(), base, block_words_);
+      blocks(pairs.data(), params.ptr, param_words_);
+      for (size_t i = 0; i < ring; i++) {
+        const uint32_t pair = pairs[i / 32], code = codes[i / 8] >> ((i / 2 % 4) * 4 + (i % 2) * 16) & 15u;
+        dst[i] = std::fma(host_half_to_float((uint16_t)pair), (float)code, host_half_to_float((uint16_t)(pair >> 16)));
+      }
+      return;
+    }
+    std::vector<uint16_t> h(ring);
+    blocks(h.data(), base, block_words_);
+    for (size_t i = 0; i < ring; i++) {
+      if (type == ST_TYPE_F16) {
+        dst[i] = host_half_to_float(h[i]);
+      } else {
+        const uint32_t u = (uint32_t)h[i] << 16;
+        std::memcpy(dst + i, &u, 4);
+      }
     }
   };
-  download(args_.keys, keys);
-  download(args_.values, values);
+  download(args_.keys, key_params_, keys);
+  download(args_.values, value_params_, values);
   if (hidden)
     HIP_CHECK(hipMemcpy(hidden, args_.hidden + (size_t)stream * c_.layers * c_.width, (size_t)c_.layers * c_.width * 4,
                         hipMemcpyDeviceToHost));

@@ -9,9 +9,11 @@
 
 #include "host_common.hpp"
 #include "batch_kernels.hpp"
+#include "cache_api.hpp"
 
 #include <cstddef>
 #include <cstdint>
+#include <vector>
 
 namespace stamd {
 
@@ -28,7 +30,8 @@ class BatchBase {
 
 class Batch : public BatchBase {
  public:
-  Batch(const st_config& config, bool mixed, const st_tensor* tensors, size_t count, int streams, int weight_dtype);
+  Batch(const st_config& config, bool mixed, const st_tensor* tensors, size_t count, int streams,
+        const st_batch_options& options);
   ~Batch() override;
   void step(const float* inputs, float* scores) override;
   void reset(int stream) override;
@@ -44,6 +47,8 @@ class Batch : public BatchBase {
   }
   template <int P> void launch_sequence();
   template <int P, bool kNT> void attend(int layer);
+  template <int P> void attend_cache(int layer);
+  void build_cache(const st_tensor* tensors, size_t count);
   // Chunks of the attention window, and whether they are spread over workgroups (batch_attention).
   // (stream, head) pairs whose chunks are split: fewer than kSplitPairs, or, of three chunks or more, between
   // one per CU and kSpillPairs (attend).
@@ -69,6 +74,16 @@ class Batch : public BatchBase {
   void sync() { HIP_CHECK(hipStreamSynchronize(stream_)); }
 
   st_config c_;
+  st_batch_options options_;
+  // Sinks, head norms or another K/V type than the model's: the cache operators take the place of the QKV epilogue
+  // and batch_attention, over caches [L][B][H][sinks + window][dh].
+  bool cached_ = false;
+  int slots_ = 0, kv_type_ = ST_TYPE_F32;
+  std::vector<st_kv_cache> caches_;
+  st_attention_args attention_{};
+  st_append_args append_{};
+  DeviceBuffer qkv_, key_params_, value_params_, gains_, workspace_;
+  size_t param_words_ = 0;  // of one (layer, stream) block of the 4-bit rows' scales and minimums
   int prec_ = kFp32, streams_ = 1, streams_p_ = 16, dim_ = 0;
   StreamHandle stream_;
   GraphHandle graph_;

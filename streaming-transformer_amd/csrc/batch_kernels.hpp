@@ -116,7 +116,8 @@ __host__ __device__ __forceinline__ size_t half_index(int b, int n, int cols) {
   return (((size_t)(b >> 4) * (cols >> 5) + (n >> 5)) * 64 + (b & 15) + 16 * (kk >> 3)) * 8 + (kk & 7);
 }
 
-enum BatchEpilogue : int { kEpInput = 0, kEpQkv, kEpOut, kEpGateUp, kEpDown };
+// kEpQkvRows: the projected rows as they are, row-major (the cache operators norm, rotate and append them).
+enum BatchEpilogue : int { kEpInput = 0, kEpQkv, kEpOut, kEpGateUp, kEpDown, kEpQkvRows };
 
 // The exact three-term bfloat16 split of FP32 values, x = hi + mid + lo: truncations, hi keeps
 // the top 8 significand bits, mid the next 8 of the remainder, lo the rest (at most 8 bits).
@@ -243,7 +244,7 @@ __global__ __launch_bounds__(64 * kSlices) void batch_proj(const char* __restric
   // buffer, in the buffer's own order (four columns of a row, then the 16 rows), so that a wave
   // stores (and loads the residual as) contiguous 256-byte runs; for QKV, whose outputs are
   // row-major, a row's pairs are consecutive.
-  constexpr int unit = (E == kEpQkv || E == kEpGateUp) ? 2 : 1;
+  constexpr int unit = (E == kEpQkv || E == kEpQkvRows || E == kEpGateUp) ? 2 : 1;
   constexpr int per_row = kBatchTile * CT / unit;
   constexpr int kUnits = NT * kBatchTile * per_row;
   constexpr int kOwn = (kUnits + kBlock - 1) / kBlock;
@@ -253,7 +254,7 @@ __global__ __launch_bounds__(64 * kSlices) void batch_proj(const char* __restric
   auto unit_of = [&](int u) {
     int o = (int)threadIdx.x + u * kBlock;
     if (kUnits % kBlock != 0 && o >= kUnits) o = kUnits - 1;
-    if constexpr (E == kEpQkv) return Unit{o / (kBatchTile * per_row), (o / per_row) % kBatchTile, (o % per_row) * unit};
+    if constexpr (E == kEpQkv || E == kEpQkvRows) return Unit{o / (kBatchTile * per_row), (o / per_row) % kBatchTile, (o % per_row) * unit};
     else return Unit{o / (kBatchTile * per_row), (o >> 2) % kBatchTile, ((o / 64) % (per_row / 4) * 4 + (o & 3)) * unit};
   };
   auto owned = [&](int u) { return kUnits % kBlock == 0 || (int)threadIdx.x + u * kBlock < kUnits; };
@@ -299,7 +300,7 @@ __global__ __launch_bounds__(64 * kSlices) void batch_proj(const char* __restric
         cs[u] = __builtin_bit_cast(v2f, gload8(rope + (size_t)b * (dim / 2) + (n0 + o.cc) % dim / 2));
         slot[u] = in_global(slots)[b];
       }
-    } else if constexpr (E == kEpGateUp) {
+    } else if constexpr (E == kEpGateUp || E == kEpQkvRows) {
       if constexpr (kScale) {
         epsilon = a.epsilon;
         asm volatile("" ::"s"(epsilon));
@@ -634,6 +635,8 @@ __global__ __launch_bounds__(64 * kSlices) void batch_proj(const char* __restric
       } else {
         *in_global(reinterpret_cast<v2f*>(base + dst)) = v2f{va, vb};
       }
+    } else if constexpr (E == kEpQkvRows) {
+      *in_global(reinterpret_cast<v2f*>(reinterpret_cast<float*>(out) + (size_t)b * out_ld + n)) = v2f{s0, s1};
     } else if constexpr (E == kEpOut) {
       const float v = cast<P>(res[u] + s0);
       reinterpret_cast<float*>(out)[act_index<P>(b, n, out_ld)] = v;
@@ -1200,6 +1203,14 @@ static __global__ void batch_reset(const BatchArgs* __restrict__ ap, int stream,
   for (size_t i = (size_t)b0 * hper + tid; i < (size_t)b1 * hper; i += step) a.hidden[i] = 0.f;
   if (tid == 0)
     for (int b = b0; b < b1; b++) a.position[b] = 0;
+}
+
+// The blocks of `words` words of one stream (all when -1) in every layer of a [layers][streams][words] array: zeros.
+static __global__ void batch_clear(unsigned* data, int layers, int streams, int stream, size_t words) {
+  const int b0 = stream < 0 ? 0 : stream, count = stream < 0 ? streams : 1;
+  const size_t span = (size_t)count * words, step = (size_t)gridDim.x * blockDim.x;
+  for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < (size_t)layers * span; i += step)
+    data[(i / span * streams + b0) * words + i % span] = 0u;
 }
 
 }  // namespace stamd

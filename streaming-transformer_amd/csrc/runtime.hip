@@ -1844,13 +1844,38 @@ struct st_batch {
   std::unique_ptr<stamd::BatchBase> impl;
 };
 
+void st_batch_options_default(st_batch_options* o) {
+  if (o) *o = st_batch_options{ST_WEIGHTS_AS_MODEL, 0, 0, ST_KV_AS_MODEL};
+}
+
+int st_batch_create_with(const st_config* config, int32_t mixed, const st_tensor* tensors, size_t count, int32_t streams,
+                         const st_batch_options* options, st_batch** out) {
+  return guarded([&] {
+    if (!config || !tensors || !out) throw stamd::Error(ST_ERR_INVALID, "Null argument");
+    *out = nullptr;
+    st_batch_options o;
+    if (options) o = *options;
+    else st_batch_options_default(&o);
+    if (options && !o.head_norm)  // a checkpoint with head norms is another model without them
+      for (size_t i = 0; i < count; i++)
+        if (tensors[i].name && std::string(tensors[i].name) == "layers.0.q_norm")
+          throw stamd::Error(ST_ERR_INVALID, "The checkpoint has head norms: set head_norm");
+    auto r = std::make_unique<st_batch>();
+    r->impl = std::make_unique<stamd::Batch>(*config, mixed != 0, tensors, count, streams, o);
+    *out = r.release();
+  });
+}
+
 int st_batch_create(const st_config* config, int32_t mixed, const st_tensor* tensors, size_t count, int32_t streams,
                     int32_t weight_dtype, st_batch** out) {
   return guarded([&] {
     if (!config || !tensors || !out) throw stamd::Error(ST_ERR_INVALID, "Null argument");
     *out = nullptr;
+    st_batch_options o;
+    st_batch_options_default(&o);
+    o.weight_dtype = weight_dtype;
     auto r = std::make_unique<st_batch>();
-    r->impl = std::make_unique<stamd::Batch>(*config, mixed != 0, tensors, count, streams, weight_dtype);
+    r->impl = std::make_unique<stamd::Batch>(*config, mixed != 0, tensors, count, streams, o);
     *out = r.release();
   });
 }

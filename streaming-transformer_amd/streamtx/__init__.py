@@ -9,8 +9,8 @@ streamtx.build    hipcc build of libstamd.so for gfx950
 from .cache import KvCache, qk_norm_rope_append, window_attention
 from .model import (Checkpoint, ModelConfig, load_checkpoint, round_bf16, round_half, synthetic_checkpoint,
                     tensor_names, write_checkpoint)
-from .runtime import Backend, BatchRuntime, Runtime, RuntimeOptions, WeightStorage, library, probe, transport_bench
+from .runtime import Backend, BatchOptions, BatchRuntime, KvStorage, Runtime, RuntimeOptions, WeightStorage, library, probe, transport_bench
 
-__all__ = ['Backend', 'BatchRuntime', 'Checkpoint', 'KvCache', 'ModelConfig', 'Runtime', 'RuntimeOptions', 'WeightStorage', 'library',
+__all__ = ['Backend', 'BatchOptions', 'BatchRuntime', 'Checkpoint', 'KvCache', 'KvStorage', 'ModelConfig', 'Runtime', 'RuntimeOptions', 'WeightStorage', 'library',
            'load_checkpoint', 'probe', 'qk_norm_rope_append', 'transport_bench', 'window_attention', 'round_bf16', 'round_half', 'synthetic_checkpoint', 'tensor_names',
            'write_checkpoint']

@@ -58,8 +58,9 @@ class ModelConfig:
         return asdict(self)
 
 
-def tensor_names(config: ModelConfig) -> list[tuple[str, tuple[int, ...]]]:
-    """Tensor names and shapes in checkpoint order (reference/model.py:27-47)."""
+def tensor_names(config: ModelConfig, head_norm: bool = False) -> list[tuple[str, tuple[int, ...]]]:
+    """Tensor names and shapes in checkpoint order (reference/model.py:27-47); with head_norm also the gains of
+    each layer's query and key norms (an extension, for BatchOptions.head_norm)."""
     c = config
     out = [('input', (c.width, c.features))]
     for layer in range(c.layers):
@@ -68,6 +69,8 @@ def tensor_names(config: ModelConfig) -> list[tuple[str, tuple[int, ...]]]:
         out += [(p + n, (c.width, c.width)) for n in ('q', 'k', 'v', 'out')]
         out += [(p + 'gate', (c.ffn, c.width)), (p + 'up', (c.ffn, c.width)), (p + 'down', (c.width, c.ffn))]
     out += [('final_norm', (c.width,)), ('score', (1, c.width))]
+    if head_norm:
+        out += [(f'layers.{layer}.{n}', (c.dim,)) for layer in range(c.layers) for n in ('q_norm', 'k_norm')]
     return out
 
 
@@ -117,7 +120,7 @@ def load_checkpoint(path) -> Checkpoint:
         end += nbytes
     if end != len(raw):
         raise ValueError('Trailing tensor bytes')
-    for name, shape in tensor_names(config):
+    for name, shape in tensor_names(config, 'layers.0.q_norm' in tensors):
         if name not in tensors or tensors[name].shape != shape:
             raise ValueError(f'Shape mismatch: {name}')
     return Checkpoint(config, mode == 'mixed', tensors, manifest)
@@ -130,7 +133,7 @@ def write_checkpoint(path, config: ModelConfig, tensors: dict, mixed: bool = Fal
     data = bytearray()
     manifest = dict(version=1, byte_order='little', orientation='out_in', config=config.to_json(),
                     mode='mixed' if mixed else 'fp32', **extra, tensors=[])
-    for name, _shape in tensor_names(config):
+    for name, _shape in tensor_names(config, 'layers.0.q_norm' in tensors):
         a = np.ascontiguousarray(tensors[name], dtype='<f2' if mixed else '<f4')
         raw = a.tobytes()
         manifest['tensors'].append(dict(name=name, shape=list(a.shape), dtype=str(a.dtype.name),

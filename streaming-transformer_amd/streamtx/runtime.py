@@ -55,6 +55,30 @@ class RuntimeOptions:
     initial_epoch: int = 0  # first epoch of the device's tagged dataflow (0 = 1); tests only
 
 
+class KvStorage(enum.IntEnum):
+    """What a batch keeps K and V in (st_batch_options.kv_dtype)."""
+    AS_MODEL = -1
+    F32 = 0
+    F16 = 1
+    BF16 = 2
+    INT4 = 3
+
+
+@dataclass
+class BatchOptions:
+    """st_batch_options: weight storage, the first events of a stream that stay visible (sinks), norms of each
+    query and key head (tensors ``layers.{l}.q_norm`` and ``.k_norm``), and the K/V storage."""
+    weight_dtype: WeightStorage = WeightStorage.AS_MODEL
+    sinks: int = 0
+    head_norm: bool = False
+    kv_dtype: KvStorage = KvStorage.AS_MODEL
+
+
+class _BatchOptions(ctypes.Structure):
+    _fields_ = [('weight_dtype', ctypes.c_int32), ('sinks', ctypes.c_int32), ('head_norm', ctypes.c_int32),
+                ('kv_dtype', ctypes.c_int32)]
+
+
 class _Config(ctypes.Structure):
     _fields_ = [('layers', ctypes.c_int32), ('width', ctypes.c_int32), ('heads', ctypes.c_int32),
                 ('ffn', ctypes.c_int32), ('window', ctypes.c_int32), ('features', ctypes.c_int32),
@@ -114,6 +138,10 @@ def library(path: os.PathLike | None = None) -> ctypes.CDLL:
     lib.st_batch_create.argtypes = [ctypes.POINTER(_Config), ctypes.c_int32, ctypes.POINTER(_Tensor),
                                     ctypes.c_size_t, ctypes.c_int32, ctypes.c_int32, ctypes.POINTER(P)]
     lib.st_batch_create_resident.argtypes = lib.st_batch_create.argtypes
+    lib.st_batch_create_with.argtypes = [ctypes.POINTER(_Config), ctypes.c_int32, ctypes.POINTER(_Tensor),
+                                         ctypes.c_size_t, ctypes.c_int32, ctypes.POINTER(_BatchOptions), ctypes.POINTER(P)]
+    lib.st_batch_options_default.argtypes = [ctypes.POINTER(_BatchOptions)]
+    lib.st_batch_options_default.restype = None
     lib.st_batch_destroy.argtypes = [P]
     lib.st_batch_destroy.restype = None
     lib.st_batch_step.argtypes = [P, F, F]
@@ -125,7 +153,7 @@ def library(path: os.PathLike | None = None) -> ctypes.CDLL:
     lib.st_window_attention.argtypes = [P, P, P, P]
     lib.st_window_attention_workspace.argtypes = [P, P, ctypes.c_int32, ctypes.c_int32, ctypes.POINTER(ctypes.c_size_t)]
     for name in ('st_qk_norm_rope_append', 'st_window_attention', 'st_window_attention_workspace',
-                 'st_batch_create', 'st_batch_create_resident', 'st_batch_step', 'st_batch_reset', 'st_batch_snapshot',
+                 'st_batch_create', 'st_batch_create_with', 'st_batch_create_resident', 'st_batch_step', 'st_batch_reset', 'st_batch_snapshot',
                  'st_batch_device_run', 'st_batch_set_eager',
                  'st_runtime_create', 'st_runtime_step', 'st_runtime_reset', 'st_runtime_stop',
                  'st_runtime_snapshot', 'st_runtime_device_trace', 'st_runtime_device_trace_noalloc',
@@ -373,9 +401,13 @@ class BatchRuntime:
     ``resident=False``: a graph of phase kernels with MFMA projections over the streams
     (1..256 streams; every stream's results bit-identical for any batch size).
     ``resident=True``: one launch of the fused step per step, each stream on its own share
-    of the CUs (1..32 streams; every stream's results bit-identical to a FUSED Runtime's)."""
+    of the CUs (1..32 streams; every stream's results bit-identical to a FUSED Runtime's).
 
-    def __init__(self, model, streams: int, weight_dtype: int = 0, resident: bool = False):
+    ``options`` (BatchOptions, not with ``resident`` or ``weight_dtype``): sinks, head norms and K/V storage of an
+    FP32 checkpoint; snapshots then hold sinks + window slots."""
+
+    def __init__(self, model, streams: int, weight_dtype: int = 0, resident: bool = False,
+                 options: BatchOptions | None = None):
         if isinstance(model, Checkpoint):
             config, tensors, mixed = model.config, model.tensors, model.mixed
         else:
@@ -384,9 +416,18 @@ class BatchRuntime:
         self.streams = int(streams)
         cfg, keep, array = _marshal(config, tensors)
         handle = ctypes.c_void_p()
-        create = library().st_batch_create_resident if resident else library().st_batch_create
-        _check(create(ctypes.byref(cfg), int(bool(mixed)), array, len(array), self.streams, int(weight_dtype),
-                      ctypes.byref(handle)))
+        self.sinks = 0
+        if options is not None:
+            if resident or weight_dtype:
+                raise ValueError('options hold the weight storage, and go with phase-kernel batches only')
+            o = _BatchOptions(int(options.weight_dtype), int(options.sinks), int(options.head_norm), int(options.kv_dtype))
+            _check(library().st_batch_create_with(ctypes.byref(cfg), int(bool(mixed)), array, len(array), self.streams,
+                                                  ctypes.byref(o), ctypes.byref(handle)))
+            self.sinks = int(options.sinks)
+        else:
+            create = library().st_batch_create_resident if resident else library().st_batch_create
+            _check(create(ctypes.byref(cfg), int(bool(mixed)), array, len(array), self.streams, int(weight_dtype),
+                          ctypes.byref(handle)))
         self.resident = bool(resident)
         self._h = handle
         self._scores = np.zeros(self.streams, dtype=np.float32)
@@ -426,9 +467,9 @@ class BatchRuntime:
         _check(library().st_batch_reset(self._handle(), int(stream)))
 
     def snapshot(self, stream: int):
-        """Runtime.snapshot() of one stream."""
+        """Runtime.snapshot() of one stream (keys and values of sinks + window slots)."""
         c = self.config
-        keys = np.empty((c.layers, c.heads, c.window, c.dim), dtype=np.float32)
+        keys = np.empty((c.layers, c.heads, self.sinks + c.window, c.dim), dtype=np.float32)
         values = np.empty_like(keys)
         hidden = np.empty((c.layers, c.width), dtype=np.float32)
         pos = ctypes.c_uint64(0)
