@@ -512,6 +512,14 @@ constexpr int wave_tile() {
   return M == kTF32 ? (D == 64 ? 32 : 16) : (D == 64 ? 64 : 32);
 }
 
+// 16 bytes of a cache row. kNT: non-temporal, for caches that the Infinity Cache does not hold: each row is read
+// once per call then, and keeping it would cost more than it gives.
+template <bool kNT>
+__device__ __forceinline__ word4_t load_row(const char* p) {
+  typedef const __attribute__((address_space(1))) word4_t* global;
+  return kNT ? __builtin_nontemporal_load((global)p) : *(global)p;
+}
+
 // The address of a pair of 16-byte (four FP32 or eight 16-bit) elements of the output row of (token row,
 // head h), elements d ..: four consecutive FP32 elements are consecutive in every layout.
 template <int A>
@@ -538,7 +546,7 @@ __device__ __forceinline__ void store_out(const AttentionView& a, int row, int h
 // A masked key's weight is an exact zero, but zero times a value that is not finite is NaN: tiles that are
 // not seen whole look for such values as they are staged, and where there is one they are added apart, for
 // the rows that see them (TileMath::add_odd).
-template <int A, int C, int D, int MB, int kWaves>
+template <int A, int C, int D, int MB, int kWaves, bool kNT>
 __global__ __launch_bounds__(64 * kWaves, 2 * 4 / kWaves) void cache_attention(CacheView c, RowsView r, AttentionView a) {
   constexpr int M = mfma_type<A, C>();
   constexpr int KT = wave_tile<M, D>();
@@ -583,24 +591,26 @@ __global__ __launch_bounds__(64 * kWaves, 2 * 4 / kWaves) void cache_attention(C
   const char* vpbase = C == kTInt4 ? reinterpret_cast<const char*>(c.value_params) + base_row * (c.row_bytes / 4) : nullptr;
   const uint32_t slot_bytes = c.slot_stride * c.row_bytes, chunk = keep ? p * 16 : 0, pair = keep ? p : 0;
   const bool near = slot_bytes < 1u << 25;  // a tile's rows within 32 bits of its first
-  word4_t kw[kLoads], vw[kLoads];
-  unsigned kp[kLoads], vp[kLoads];
+  struct Loaded {
+    word4_t kw[kLoads], vw[kLoads];
+    unsigned kp[kLoads], vp[kLoads];
+  };
   // The loads have one place and no condition: a branch around them, or two forms of them, makes the compiler
   // move what they return, which waits for it. Those past the last tile repeat it.
   const uint32_t part = sub * slot_bytes;
-  auto load = [&](int j0) {
+  auto load = [&](int j0, Loaded& t) {
     uint64_t at[kLoads];
     keys.offsets(j0, kPerLoad, sub, KT, near, slot_bytes, part, at);
 #pragma unroll
-    for (int i = 0; i < kLoads; i++) kw[i] = load_global<word4_t>(kbase + at[i] + chunk);
+    for (int i = 0; i < kLoads; i++) t.kw[i] = load_row<kNT>(kbase + at[i] + chunk);
 #pragma unroll
-    for (int i = 0; i < kLoads; i++) vw[i] = load_global<word4_t>(vbase + at[i] + chunk);
+    for (int i = 0; i < kLoads; i++) t.vw[i] = load_row<kNT>(vbase + at[i] + chunk);
     if constexpr (C == kTInt4) {
 #pragma unroll
       for (int i = 0; i < kLoads; i++) {
         const uint64_t params = at[i] / 16 * 4 + pair * 4;  // 16 bytes of codes have 4 of scale and minimum
-        kp[i] = load_global<unsigned>(kpbase + params);
-        vp[i] = load_global<unsigned>(vpbase + params);
+        t.kp[i] = load_global<unsigned>(kpbase + params);
+        t.vp[i] = load_global<unsigned>(vpbase + params);
       }
     }
   };
@@ -608,7 +618,11 @@ __global__ __launch_bounds__(64 * kWaves, 2 * 4 / kWaves) void cache_attention(C
   const int tiles = (keys.total + KT - 1) / KT, per = (tiles + a.splits - 1) / a.splits;
   const int t1 = min((split + 1) * per, tiles);
   int tile = split * per + wave;
-  load(min(tile, tiles - 1) * KT);
+  // 4-bit tiles are a quarter of the bytes: two of them in flight per wave.
+  constexpr int kSets = C == kTInt4 ? 2 : 1;
+  Loaded loaded[kSets];
+#pragma unroll
+  for (int i = 0; i < kSets; i++) load(min(tile + i * kWaves, tiles - 1) * KT, loaded[i]);
 
   QueryBlock<A, M, D> q[MB];
   Seen seen[MB];
@@ -629,7 +643,7 @@ __global__ __launch_bounds__(64 * kWaves, 2 * 4 / kWaves) void cache_attention(C
   const int whole_to = keys.sinks + max((int)max(ta - keys.lo, (int64_t)-1) + 1, 0);
   const int whole_sinks = (int)min((int64_t)keys.sinks, ta + 1);
 
-  for (; tile < t1; tile += kWaves) {
+  auto step = [&](int tile, Loaded& in) {
     const int j0 = tile * KT;
     // Whole: every row sees the tile's every entry.
     const bool whole = (j0 >= whole_from && j0 + KT <= whole_to) || j0 + KT <= whole_sinks ||
@@ -639,8 +653,8 @@ __global__ __launch_bounds__(64 * kWaves, 2 * 4 / kWaves) void cache_attention(C
 #pragma unroll
     for (int i = 0; i < kLoads; i++) {
       const int row = i * kPerLoad + sub;
-      expand<C, M>(kw[i], kp[i], p, keep, [&](int ch, word4_t w) { lds_put(kt + row * T::kRow + T::key_chunk(row, ch) * 16, w); });
-      expand<C, M>(vw[i], vp[i], p, keep, [&](int ch, word4_t w) {
+      expand<C, M>(in.kw[i], in.kp[i], p, keep, [&](int ch, word4_t w) { lds_put(kt + row * T::kRow + T::key_chunk(row, ch) * 16, w); });
+      expand<C, M>(in.vw[i], in.vp[i], p, keep, [&](int ch, word4_t w) {
         lds_put(vt + row * T::kRow + T::value_chunk(row, ch) * 16, w);
         if (!whole) odd |= not_finite<M>(w);
       });
@@ -660,15 +674,21 @@ __global__ __launch_bounds__(64 * kWaves, 2 * 4 / kWaves) void cache_attention(C
 #pragma unroll
       for (int i = 0; i < kLoads; i++) {
         const int row = i * kPerLoad + sub;
-        expand<C, M, 1>(kw[i], kp[i], p, keep, [&](int ch, word4_t w) { lds_put(kt + row * T::kRow + T::key_chunk(row, ch) * 16, w); });
+        expand<C, M, 1>(in.kw[i], in.kp[i], p, keep, [&](int ch, word4_t w) { lds_put(kt + row * T::kRow + T::key_chunk(row, ch) * 16, w); });
       }
       wave_sync();
     }
-    load(min(tile + kWaves, t1 - 1) * KT);
+    load(min(tile + kSets * kWaves, t1 - 1) * KT, in);
     X::template logits<two_terms<A, C>()>(kt, q, s, lane);
     if (!whole) X::mask(s, seen, keys, c.window, j0, lane);
     move_maxima(s, q, m, base, o);
     X::outputs(vt, s, q, base, o, lane);
+  };
+  for (; tile < t1; tile += kSets * kWaves) {
+    step(tile, loaded[0]);
+    if constexpr (kSets > 1) {
+      if (tile + kWaves < t1) step(tile + kWaves, loaded[1]);
+    }
   }
 
   // Merge of the four waves.
@@ -732,7 +752,7 @@ constexpr int vector_loads() {  // loads of K (and of V) in flight per wave
   return C == kTInt4 ? 2 : 8;
 }
 constexpr int kVectorWaves = 8;
-template <int C, int D, int R>
+template <int C, int D, int R, bool kNT>
 __global__ __launch_bounds__(64 * kVectorWaves) void cache_attention_vector(CacheView c, RowsView r, AttentionView a) {
   using Row = RowLoad<C, D>;
   constexpr int E = Row::E, L = Row::L, kGroups = 64 / L, NB = vector_loads<C, D>(), KT = NB * kGroups;
@@ -777,14 +797,14 @@ __global__ __launch_bounds__(64 * kVectorWaves) void cache_attention_vector(Cach
   auto load_keys = [&] {
 #pragma unroll
     for (int i = 0; i < NB; i++) {
-      kw[i] = load_global<word4_t>(kbase + at[i]);
+      kw[i] = load_row<kNT>(kbase + at[i]);
       if constexpr (C == kTInt4) kp[i] = load_global<unsigned>(kpbase + at[i] / 16 * 4);
     }
   };
   auto load_values = [&] {
 #pragma unroll
     for (int i = 0; i < NB; i++) {
-      vw[i] = load_global<word4_t>(vbase + at[i]);
+      vw[i] = load_row<kNT>(vbase + at[i]);
       if constexpr (C == kTInt4) vp[i] = load_global<unsigned>(vpbase + at[i] / 16 * 4);
     }
   };
@@ -981,14 +1001,14 @@ void cache_attention_rows(CacheView c, RowsView r, AttentionView a) {
   static_assert(!kDirect || KT % kPerLoad == 0);
   __shared__ __attribute__((aligned(16))) char lds[2][kTwo ? 3 : 2][kTile];
 
-  const int head = blockIdx.x % c.kv_heads, b = blockIdx.y;
+  const int split = blockIdx.x % a.splits, head = blockIdx.x / a.splits % c.kv_heads, b = blockIdx.y;
   const int64_t start = uniform64(c.positions[b]);
   int first, n;
   stream_rows(r, b, first, n);
   first = __builtin_amdgcn_readfirstlane(first);
   n = __builtin_amdgcn_readfirstlane(n);
   const int rows = n * a.group, tiles_of_rows = (rows + kRows - 1) / kRows;
-  const int tile_of_rows = tiles_of_rows - 1 - (int)(blockIdx.x / c.kv_heads);
+  const int tile_of_rows = tiles_of_rows - 1 - (int)(blockIdx.x / a.splits / c.kv_heads);
   if (start < 0 || tile_of_rows < 0) return;
   const int row0 = tile_of_rows * kRows, last_row = min(row0 + kRows, rows) - 1;
   KeyList keys;
@@ -1065,8 +1085,9 @@ void cache_attention_rows(CacheView c, RowsView r, AttentionView a) {
     __syncthreads();
   }
 
-  const int tiles = (keys.total + KT - 1) / KT;
-  load(0, 0);
+  const int all_tiles = (keys.total + KT - 1) / KT, per = (all_tiles + a.splits - 1) / a.splits;
+  const int begin = min(split * per, all_tiles), tiles = min(begin + per, all_tiles);  // this split's: begin .. tiles - 1
+  if (begin < tiles) load(begin * KT, begin & 1);
   QueryBlock<A, M, D> q[MB];
   Seen seen[MB];
   float m[MB];
@@ -1093,7 +1114,8 @@ void cache_attention_rows(CacheView c, RowsView r, AttentionView a) {
   const int all_from = keys.sinks + max(keys.total - keys.sinks - c.window, 0);
   const int all_to = keys.sinks + (int)max(start + row0 / a.group - keys.lo, (int64_t)-1) + 1;
   auto partial = [&](int j0) { return !(j0 >= all_from && j0 + KT <= all_to); };
-  bool odd = __syncthreads_or(stage(0, partial(0))) != 0;
+  bool odd = false;
+  if (begin < tiles) odd = __syncthreads_or(stage(begin & 1, partial(begin * KT))) != 0;
 
   // One tile. kWhole: all of the workgroup's rows see all of it.
   auto step = [&](int tile, auto kWhole) {
@@ -1136,8 +1158,8 @@ void cache_attention_rows(CacheView c, RowsView r, AttentionView a) {
   };
   // The tiles seen whole are one run: a loop of their own, in which nothing branches around the products (a
   // branch around the masks alone cost a register move per logit).
-  const int run_from = min((all_from + KT - 1) / KT, tiles), run_to = max(run_from, all_to / KT);
-  int tile = 0;
+  const int run_from = max(min((all_from + KT - 1) / KT, tiles), begin), run_to = max(run_from, min(all_to / KT, tiles));
+  int tile = begin;
   for (int round = 0; round < 2; round++) {
     const int until = round ? tiles : run_from;
     for (; tile < until; tile++) step(tile, std::false_type{});
@@ -1146,9 +1168,15 @@ void cache_attention_rows(CacheView c, RowsView r, AttentionView a) {
 
 #pragma unroll
   for (int u = 0; u < MB; u++) {
-    const float inv = 1.f / X::row_sum(o[u][D / 16]);
+    const float sum = X::row_sum(o[u][D / 16]), inv = 1.f / sum;
     const int row = wave_row0 + u * 16 + (lane & 15);
-    if (row <= last_row) {
+    if (row <= last_row && a.splits > 1) {
+      const size_t at = (((size_t)b * c.kv_heads + head) * a.rows + row) * a.splits + split;
+      if (g == 0) a.part_ml[at] = make_float2(m[u], sum);
+#pragma unroll
+      for (int d = 0; d < D / 16; d++)
+        if (d * 16 + g * 4 < c.dim) store_global(a.part_o + at * c.dim + d * 16 + g * 4, o[u][d]);
+    } else if (row <= last_row) {
       const int token = row / a.group, h = head * a.group + row - token * a.group;
 #pragma unroll
       for (int d = 0; d < D / 16; d++) {

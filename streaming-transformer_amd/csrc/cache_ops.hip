@@ -59,6 +59,19 @@ void check_heads(const st_kv_cache* cache, const st_new_rows* rows, int q_heads)
 // Head dimension of the kernels: the smallest that holds it.
 int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
+// cache_attention_rows is taken where it has kManyWaves waves, which is half of what the chip holds, by itself or
+// split along the keys into shares of kManyKeys or more. us of cache_attention (split) / cache_attention_rows, 32
+// heads on 8, head dimension 128, bfloat16: 128 tokens and a window of 1024, one stream 25 / 34 (128 waves), four
+// 34 / 35 (512), 16 118 / 54 (2048); window 8192, one stream 57 / 45 (128 waves x 8 splits), four 168 / 101 (512 x
+// 4), 16 621 / 306; one stream of 512 tokens 158 / 97. Over 4-bit rows, eight streams, window 2048: 32 tokens 41 /
+// 54 (512 waves x 2), 128 tokens 100 / 83 (1024).
+// Rows per (stream, cache head) above which: a wave of theirs has 32, so fewer leave waves idle, and FP32 products
+// or converted rows cost those that work more. 64 streams, window 1024, 32 rows 52 / 55, 36 rows 65 / 52; 4-bit 96
+// rows 92 / 97, 128 rows 115 / 95; FP32 (32 streams, window 512) 64 rows 71 / 103, 128 rows 130 / 114.
+constexpr int kManyRows = 32, kManyRowsSlow = 96;
+constexpr int kManyWaves = 1024, kManySplit = 2048, kManyKeys = 1024;
+constexpr size_t kStreamBytes = (size_t)256 << 20;  // the Infinity Cache
+
 struct Plan {
   bool many;   // cache_attention_rows
   int vector;  // rows of cache_attention_vector; 0, and not many: cache_attention
@@ -66,29 +79,34 @@ struct Plan {
   int waves;   // of a workgroup
   int tiles;   // row tiles of a (stream, kv head)
   int splits;
+  bool stream;  // non-temporal loads (decoding)
 };
 Plan plan_attention(const CacheView& c, const RowsView& r, int q_heads, int dtype, int stored) {
   Plan p{};
   const int rows = r.max_tokens * (q_heads / c.kv_heads), padded = padded_dim(c.dim);
+  const int64_t pairs = (int64_t)c.streams * c.kv_heads;
+  const int64_t keys = (int64_t)c.sinks + std::min<int64_t>(c.ring, (int64_t)c.window + r.max_tokens - 1);
+  if (rows > (dtype != ST_TYPE_F32 && dtype == stored ? kManyRows : kManyRowsSlow)) {
+    const int waves = rows_waves(dtype, stored, padded), blocks = padded == 256 ? 1 : 2, tile = 16 * blocks * waves;
+    p.tiles = (rows + tile - 1) / tile;
+    const int64_t base = pairs * p.tiles, splits = std::min<int64_t>({kManySplit / (base * waves), keys / kManyKeys, kMaxSplits});
+    if (base * waves >= kManyWaves || (splits >= 4 && base * waves * splits >= kManyWaves)) {
+      p.many = true;
+      p.blocks = blocks;
+      p.splits = (int)std::max<int64_t>(1, splits);
+      return p;
+    }
+  }
   p.blocks = rows > 16 && padded < 256 ? 2 : 1;  // head dimension 256: one block's registers fill the file
   p.tiles = (rows + 16 * p.blocks - 1) / (16 * p.blocks);
-  const int64_t pairs = (int64_t)c.streams * c.kv_heads;
-  if (rows > 64) {
-    p.many = true;
-    p.blocks = padded == 256 ? 1 : 2;
-    const int tile = 16 * p.blocks * rows_waves(dtype, stored, padded);
-    p.tiles = (rows + tile - 1) / tile;
-    p.splits = 1;
-    return p;
-  }
   const int group = q_heads / c.kv_heads;
   // Four query heads over 4-bit rows, 32 elements of each to a lane, do not fit into registers.
   if (dtype == ST_TYPE_F32 && r.max_tokens == 1 && group <= (stored == ST_TYPE_INT4 ? 2 : 4)) p.vector = group == 3 ? 4 : group;
-  // Workgroups beside the splits, and as many as the chip holds at once (2 per CU; 1 of head dimension 256).
+  p.stream = 2 * pairs * keys * c.row_bytes > (int64_t)kStreamBytes;
+  // Workgroups beside the splits, and as many as the chip holds at once.
   const int64_t base = pairs * p.tiles;
   p.waves = p.vector || (p.blocks == 1 && padded < 256) ? 8 : 4;
   const int64_t room = padded == 256 || p.waves == 8 ? 256 : 512;
-  const int64_t keys = (int64_t)c.sinks + std::min<int64_t>(c.ring, (int64_t)c.window + r.max_tokens - 1);
   const int64_t share = p.waves * 32 * 2;  // fewest keys of a split: two tiles for each wave
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(room + base - 1) / base, keys / share, kMaxSplits}));
   return p;
@@ -115,18 +133,23 @@ void launch_attention(const CacheView& c, const RowsView& r, const AttentionView
   auto form = [&](auto D) {
     constexpr int d = decltype(D)::value;
     if (p.many) return go(cache_attention_rows<A, C, d, d == 256 ? 1 : 2>, rows_threads(A, C, d));
-    if constexpr (A == kTF32) {
-      if (p.vector == 1) return go(cache_attention_vector<C, d, 1>, 64 * kVectorWaves);
-      if (p.vector == 2) return go(cache_attention_vector<C, d, 2>, 64 * kVectorWaves);
-      if constexpr (C != kTInt4) {
-        if (p.vector == 4) return go(cache_attention_vector<C, d, 4>, 64 * kVectorWaves);
+    auto few = [&](auto NT) {
+      constexpr bool nt = decltype(NT)::value;
+      if constexpr (A == kTF32) {
+        if (p.vector == 1) return go(cache_attention_vector<C, d, 1, nt>, 64 * kVectorWaves);
+        if (p.vector == 2) return go(cache_attention_vector<C, d, 2, nt>, 64 * kVectorWaves);
+        if constexpr (C != kTInt4) {
+          if (p.vector == 4) return go(cache_attention_vector<C, d, 4, nt>, 64 * kVectorWaves);
+        }
       }
-    }
+      if constexpr (d < 256) go(cache_attention<A, C, d, 1, 8, nt>, 512);
+      else go(cache_attention<A, C, d, 1, 4, nt>, 256);
+    };
     if constexpr (d < 256) {
-      if (p.blocks == 2) return go(cache_attention<A, C, d, 2, 4>, 256);
-      if (p.waves == 8) return go(cache_attention<A, C, d, 1, 8>, 512);
+      if (p.blocks == 2) return go(cache_attention<A, C, d, 2, 4, false>, 256);
     }
-    go(cache_attention<A, C, d, 1, 4>, 256);
+    if (p.stream) few(std::true_type{});
+    else few(std::false_type{});
   };
   const int padded = padded_dim(c.dim);
   if (padded == 64) form(std::integral_constant<int, 64>{});
@@ -212,7 +235,8 @@ CacheView cache_view(const st_kv_cache* s) {
 
 RowsView rows_view(const st_kv_cache* s, const st_new_rows* rows) {
   require(rows != nullptr, "Null argument");
-  require(rows->tokens >= 0 && rows->max_tokens >= 1, "A call needs tokens >= 0 and max_tokens >= 1");
+  require(rows->tokens >= 0 && rows->tokens <= 1 << 30 && rows->max_tokens >= 1,
+          "A call needs tokens between 0 and 2^30 and max_tokens >= 1");
   require(rows->max_tokens <= s->ring - s->window + 1, "More new tokens than the ring has rows beside the window");
   require(rows->offsets || (int64_t)s->streams * rows->max_tokens == rows->tokens,
           "Without offsets every stream brings max_tokens rows");

@@ -69,7 +69,7 @@ CACHES = [
     (dict(slot_stride=1, head_stride=1, stream_stride=2**40), 'strides'),
 ]
 ROWS = [
-    (dict(tokens=-1), 'tokens'), (dict(max_tokens=0), 'tokens'), (dict(max_tokens=-5), 'tokens'),
+    (dict(tokens=-1), 'tokens'), (dict(tokens=MOST, offsets=A), 'tokens'), (dict(max_tokens=0), 'tokens'), (dict(max_tokens=-5), 'tokens'),
     (dict(tokens=3), 'Without offsets'), (dict(tokens=12, max_tokens=6), 'beside the window'),
     (dict(max_tokens=MOST), 'beside the window'), (dict(offsets=A + 2), 'offsets'),
 ]
