@@ -373,6 +373,14 @@ struct TileMath {
       }
     }
   }
+  // Whether the thread's share of a tile of V holds a value that is not finite.
+  template <int kThreads>
+  __device__ static __forceinline__ bool any_odd(const char* vt, int thread) {
+    bool found = false;
+#pragma unroll 1
+    for (int at = thread * 16; at < KT * T::kRow; at += kThreads * 16) found |= not_finite<M>(lds_load<word4_t>(vt + at));
+    return found;
+  }
   template <int kThreads>
   __device__ static __forceinline__ void clear(char* vt, int thread) {
 #pragma unroll 1
@@ -648,19 +656,15 @@ __global__ __launch_bounds__(64 * kWaves, 2 * 4 / kWaves) void cache_attention(C
     // Whole: every row sees the tile's every entry.
     const bool whole = (j0 >= whole_from && j0 + KT <= whole_to) || j0 + KT <= whole_sinks ||
                        (whole_sinks == keys.sinks && whole_from == keys.sinks && j0 + KT <= whole_to);
-    bool odd = false;  // a value that is not finite in a tile that is not whole
     wave_sync();
 #pragma unroll
     for (int i = 0; i < kLoads; i++) {
       const int row = i * kPerLoad + sub;
       expand<C, M>(in.kw[i], in.kp[i], p, keep, [&](int ch, word4_t w) { lds_put(kt + row * T::kRow + T::key_chunk(row, ch) * 16, w); });
-      expand<C, M>(in.vw[i], in.vp[i], p, keep, [&](int ch, word4_t w) {
-        lds_put(vt + row * T::kRow + T::value_chunk(row, ch) * 16, w);
-        if (!whole) odd |= not_finite<M>(w);
-      });
+      expand<C, M>(in.vw[i], in.vp[i], p, keep, [&](int ch, word4_t w) { lds_put(vt + row * T::kRow + T::value_chunk(row, ch) * 16, w); });
     }
     wave_sync();
-    if (__ballot(odd)) {
+    if (!whole && __ballot(X::template any_odd<64>(vt, lane))) {
       X::add_odd(vt, o, lane, [&](int u, int e) { return seen[u](keys, c.window, j0 + e); });
       wave_sync();
       X::template clear<64>(vt, lane);
@@ -1053,14 +1057,8 @@ void cache_attention_rows(CacheView c, RowsView r, AttentionView a) {
   };
   // Waits for the loads and stages what came to registers; look: whether any value of V is not finite.
   auto stage = [&](int buffer, bool look) {
-    bool found = false;
     if constexpr (kDirect) {
       wait_loads();
-      if (look) {
-#pragma unroll
-        for (int i = 0; i < kLoads; i++)
-          found |= not_finite<M>(lds_load<word4_t>(lds[buffer][1] + (i * kThreads + (int)threadIdx.x) * 16));
-      }
     } else {
 #pragma unroll
       for (int i = 0; i < kLoads; i++) {
@@ -1071,14 +1069,13 @@ void cache_attention_rows(CacheView c, RowsView r, AttentionView a) {
           if constexpr (kTwo)
             expand<C, M, 1>(raw[i], params[i], p, keep, [&](int ch, word4_t w) { lds_put(lds[buffer][2] + row * T::kRow + T::key_chunk(row, ch) * 16, w); });
         } else {
-          expand<C, M>(raw[i], params[i], p, keep, [&](int ch, word4_t w) {
-            lds_put(lds[buffer][1] + row * T::kRow + T::value_chunk(row, ch) * 16, w);
-            if (look) found |= not_finite<M>(w);
-          });
+          expand<C, M>(raw[i], params[i], p, keep, [&](int ch, word4_t w) { lds_put(lds[buffer][1] + row * T::kRow + T::value_chunk(row, ch) * 16, w); });
         }
       }
     }
-    return found;
+    if (!look) return false;
+    __syncthreads();
+    return X::template any_odd<kThreads>(lds[buffer][1], threadIdx.x);
   };
   if (kDirect && c.dim < D) {  // the padding, which no load writes
     for (int at = threadIdx.x * 16; at < (int)sizeof(lds); at += kThreads * 16) lds_put(&lds[0][0][0] + at, word4_t{0, 0, 0, 0});

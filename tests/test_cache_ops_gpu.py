@@ -246,6 +246,45 @@ def test_attention_long_window_is_split(dtype, stored):
     run_attention(dtype, stored, 128, 4, 1, 9000, 4, 3, [8000])
 
 
+@pytest.mark.parametrize('dtype,stored', [(BF16, BF16), (F16, INT4), (F32, F32)])
+def test_attention_many_rows_are_split(dtype, stored):
+    """Few streams, many rows and long windows: row tiles, each split over workgroups along the keys."""
+    run_attention(dtype, stored, 64, 32, 4, 8192, 4, 34, [9000, 100, 8190, -1], counts=[34, 34, 30, 0])
+
+
+def test_attention_cache_past_the_infinity_cache():
+    """A 16-bit cache of more than 256 MB, whose rows are read with non-temporal loads: values at both ends of the
+    window and at its start, all keys zero but one."""
+    dim, slots = 128, 700_000
+    rows = []
+    for _ in range(2):
+        p = ctypes.c_void_p()
+        hip().hipMalloc(ctypes.byref(p), ctypes.c_size_t(slots * dim * 2))
+        hip().hipMemset(p, 0, ctypes.c_size_t(slots * dim * 2))
+        rows.append(p)
+    from streamtx.cache import _Cache
+    cache = Cache.__new__(Cache)
+    cache.dims, cache.dim, cache.window, cache.sinks, cache.ring, cache.dtype = (1, 1, slots), dim, slots, 0, slots, BF16
+    cache.positions = Device(np.asarray([slots + 5], np.int64))
+    cache.struct = _Cache(1, 1, dim, slots, 0, slots, BF16, 0, 0, 0, rows[0].value, rows[1].value, None, None,
+                          cache.positions.ptr)
+    mark = encode(np.random.default_rng(4).standard_normal((3, dim)), BF16)
+    for m, at in zip(mark, (0, 399_999, slots - 1)):
+        hip().hipMemcpy(ctypes.c_void_p(rows[1].value + at * dim * 2), m.ctypes.data_as(ctypes.c_void_p), dim * 2, 1)
+    r, _, _ = rows_struct(cache, n=1)
+    q, k, v = (Heads(np.ones((1, n, dim)), BF16) for n in (4, 1, 1))
+    out = Heads(np.zeros((1, 4, dim)), BF16)
+    append(cache, r, q, k, v, out)
+    keep = attend(cache, r, q, out, scale=0.125)
+    e = np.exp(-16.0)
+    want = (1 + e * decode(mark, BF16).sum(0)) / (1 + e * (slots - 1))
+    # The weights' sums in FP32 (some 2000 roundings deep where a wave walks its share), then the output's rounding.
+    assert np.abs(out.get()[0] - want).max() <= (STEP[BF16] + 4096 * 2.0**-24) * np.abs(want).max()
+    for p in rows:
+        hip().hipFree(p)
+    del keep
+
+
 @pytest.mark.parametrize('dtype,stored', [(F32, F32), (F16, F16), (BF16, BF16), (F16, INT4), (BF16, INT4)])
 def test_attention_large_logits(dtype, stored):
     """Logits of a hundred and more: the running maximum carries the exponentials."""
