@@ -88,7 +88,8 @@ struct Seen {
 // A tile of K and V rows in LDS, the elements that the MFMAs take: FP32, or 16 bits. Rows are D elements
 // (the head dimension padded with zeros to 64, 128 or 256) in 16-byte chunks; chunk c of row r is stored
 // at c ^ swizzle(r), which spreads over the banks what 16 lanes read at once: one chunk of 16 rows (K),
-// 32 bytes of 16 rows (V, transposed 16-bit reads), 64 bytes of four rows (V, FP32).
+// 32 bytes of 16 rows (V, transposed 16-bit reads), 64 bytes of four rows (V, FP32); and what 16 lanes write of
+// 4-bit rows, every fourth chunk of four rows.
 template <int M, int D>
 struct TileLayout {
   static constexpr int kElem = M == kTF32 ? 4 : 2;
@@ -97,7 +98,7 @@ struct TileLayout {
   __device__ static __forceinline__ int value_chunk(int r, int c) {
     if constexpr (M == kTF32) return c ^ (((r >> 2) & 3) << 2);
     else if constexpr (kChunks == 8) return c ^ (((r >> 1) & 3) << 1);
-    else return c ^ ((r & 7) << 1);
+    else return c ^ ((r & 7) << 1 | (r >> 1 & 1));
   }
 };
 
@@ -121,8 +122,12 @@ __device__ __forceinline__ word4_t dequant8_f16(unsigned w, half2_t sz) {
     const float a = (float)code[0] * (float)sz[0] + (float)sz[1], b = (float)code[1] * (float)sz[0] + (float)sz[1];
     return pack_f16(a - (float)v[0], b - (float)v[1]);
   };
-  auto low = [&](unsigned x) { return value(__builtin_bit_cast(half2_t, (x & 0x000f000fu) | 0x64006400u) - big); };
-  auto high = [&](unsigned x) { return value(__builtin_bit_cast(half2_t, (x & 0x00f000f0u) | 0x54005400u) - mid); };
+  // The constants in registers: as literals, of which an instruction takes one, AND and OR are two instructions.
+  unsigned low_mask = 0x000f000fu, high_mask = 0x00f000f0u, low_one = 0x64006400u, high_one = 0x54005400u;
+  asm("" : "+s"(low_mask), "+s"(high_mask));
+  asm("" : "+v"(low_one), "+v"(high_one));
+  auto low = [&](unsigned x) { return value(__builtin_bit_cast(half2_t, (x & low_mask) | low_one) - big); };
+  auto high = [&](unsigned x) { return value(__builtin_bit_cast(half2_t, (x & high_mask) | high_one) - mid); };
   return word4_t{low(w), high(w), low(w >> 8), high(w >> 8)};
 }
 __device__ __forceinline__ void dequant8_f32(unsigned w, float s, float z, float4_t (&out)[2]) {
@@ -137,10 +142,8 @@ __device__ __forceinline__ void dequant8_f32(unsigned w, float s, float z, float
 // put(chunk, value) for each. `keep`: whether the lane's elements are inside the head. kTerm: of 4-bit rows.
 template <int C, int M, int kTerm = 0, typename Put>
 __device__ __forceinline__ void expand(word4_t w, unsigned params, int p, bool keep, Put&& put) {
-  if (!keep) {
-    w = word4_t{0, 0, 0, 0};
-    params = 0;
-  }
+  if constexpr (C == kTInt4) params = keep ? params : 0u;  // zeros, whatever the codes
+  else w = keep ? w : word4_t{0, 0, 0, 0};
   if constexpr (C == M) {
     put(p, w);
   } else if constexpr (C == kTInt4) {
@@ -282,8 +285,8 @@ struct QueryBlock {
 
 // Products of one tile with a block of 16 rows, for a wave. kt and vt: the tile's K and V in LDS.
 // kFine: 16-bit weights in two terms (w and what its rounding left), so that the output's own rounding is
-// the only one that counts; twice the products with V.
-template <int M, int D, int KT, bool kFine>
+// the only one that counts; twice the products with V. U: the head's dimensions that are multiplied, in steps of 32.
+template <int M, int D, int U, int KT, bool kFine>
 struct TileMath {
   using T = TileLayout<M, D>;
   static constexpr int kBlocks = KT / 16;
@@ -342,7 +345,7 @@ struct TileMath {
   // outputs of the rows that see them, before clear makes them zeros, which the products then add nothing
   // for.
   template <int MB, typename Sees>
-  __device__ static __forceinline__ void add_odd(const char* vt, float4_t (&o)[MB][D / 16 + 1], int lane, Sees&& sees) {
+  __device__ static __forceinline__ void add_odd(const char* vt, float4_t (&o)[MB][U / 16 + 1], int lane, Sees&& sees) {
     const int g = lane >> 4;
 #pragma unroll 1
     for (int r = 0; r < KT; r++) {
@@ -350,7 +353,7 @@ struct TileMath {
 #pragma unroll
       for (int u = 0; u < MB; u++) seen[u] = sees(u, r);
 #pragma unroll
-      for (int db = 0; db < D / 16; db++) {
+      for (int db = 0; db < U / 16; db++) {
         float v[4];
         if constexpr (M == kTF32) {
           const float4_t x = lds_load<float4_t>(vt + r * T::kRow + T::value_chunk(r, db * 4 + g) * 16);
@@ -403,7 +406,7 @@ struct TileMath {
   // ones (every element is the row's whole sum), for FP32 the lane's own share in four parts.
   template <int MB, typename Q>
   __device__ static __forceinline__ void outputs(const char* vt, const float4_t (&s)[MB][kBlocks], const Q (&q)[MB],
-                                                 const float (&base)[MB], float4_t (&o)[MB][D / 16 + 1], int lane) {
+                                                 const float (&base)[MB], float4_t (&o)[MB][U / 16 + 1], int lane) {
 #pragma unroll
     for (int depth = 0; depth < kDepths; depth++) {
       word4_t w[MB], rest[MB];
@@ -416,7 +419,7 @@ struct TileMath {
         if constexpr (M == kTF32) {
           const float4_t x = {p[0], p[1], p[2], p[3]};
           w[u] = __builtin_bit_cast(word4_t, x);
-          o[u][D / 16] += x;
+          o[u][U / 16] += x;
         } else {
           constexpr unsigned one = M == kTF16 ? 0x3c003c00u : 0x3f803f80u;
           const word4_t ones = {one, one, one, one};
@@ -425,12 +428,12 @@ struct TileMath {
             w[u][i] = pack16<M>(p[2 * i], p[2 * i + 1]);
             if constexpr (kFine) rest[u][i] = pack16<M>(p[2 * i] - low16<M>(w[u][i]), p[2 * i + 1] - high16<M>(w[u][i]));
           }
-          o[u][D / 16] = Mfma<M>::mul(ones, w[u], o[u][D / 16]);
-          if constexpr (kFine) o[u][D / 16] = Mfma<M>::mul(ones, rest[u], o[u][D / 16]);
+          o[u][U / 16] = Mfma<M>::mul(ones, w[u], o[u][U / 16]);
+          if constexpr (kFine) o[u][U / 16] = Mfma<M>::mul(ones, rest[u], o[u][U / 16]);
         }
       }
 #pragma unroll
-      for (int d = 0; d < D / 16; d++) {
+      for (int d = 0; d < U / 16; d++) {
         const word4_t v = values(vt, depth, d, lane);
 #pragma unroll
         for (int u = 0; u < MB; u++) o[u][d] = Mfma<M>::mul(v, w[u], o[u][d]);
@@ -561,7 +564,7 @@ __global__ __launch_bounds__(64 * kWaves, 2 * 4 / kWaves) void cache_attention(C
   using T = TileLayout<M, D>;
   using R = RowLoad<C, D>;
   // (FP16 weights are far finer than a bfloat16 output.)
-  using X = TileMath<M, D, KT, M != kTF32 && M == A>;
+  using X = TileMath<M, D, D, KT, M != kTF32 && M == A>;
   constexpr int kPerLoad = 64 / R::L;                                // rows of one load of the wave
   constexpr int kLoads = (KT + kPerLoad - 1) / kPerLoad;
   static_assert(KT % kPerLoad == 0);
@@ -987,7 +990,7 @@ constexpr int rows_tile() {
 constexpr int rows_waves(int type, int stored, int dim) { return type == stored || dim > 128 ? 4 : 8; }
 constexpr int rows_threads(int type, int stored, int dim) { return 64 * rows_waves(type, stored, dim); }
 constexpr int rows_per_cu(int type, int stored, int dim) { return dim > 128 ? 1 : 8 / rows_waves(type, stored, dim); }
-template <int A, int C, int D, int MB>
+template <int A, int C, int D, int U, int MB>
 __global__ __launch_bounds__(rows_threads(A, C, D), rows_per_cu(A, C, D))
 void cache_attention_rows(CacheView c, RowsView r, AttentionView a) {
   constexpr int M = mfma_type<A, C>();
@@ -995,7 +998,7 @@ void cache_attention_rows(CacheView c, RowsView r, AttentionView a) {
   using T = TileLayout<M, D>;
   using R = RowLoad<C, D>;
   constexpr bool kTwo = two_terms<A, C>();  // both terms of K are staged
-  using X = TileMath<M, D, KT, kTwo>;
+  using X = TileMath<M, D, U, KT, kTwo>;
   constexpr bool kDirect = C == M;
   constexpr int kWaves = rows_waves(A, C, D), kThreads = 64 * kWaves, kRows = kWaves * MB * 16;
   constexpr int kLoaders = kDirect ? kThreads : kThreads / 2;  // of one of K and V
@@ -1085,10 +1088,10 @@ void cache_attention_rows(CacheView c, RowsView r, AttentionView a) {
   const int all_tiles = (keys.total + KT - 1) / KT, per = (all_tiles + a.splits - 1) / a.splits;
   const int begin = min(split * per, all_tiles), tiles = min(begin + per, all_tiles);  // this split's: begin .. tiles - 1
   if (begin < tiles) load(begin * KT, begin & 1);
-  QueryBlock<A, M, D> q[MB];
+  QueryBlock<A, M, U> q[MB];
   Seen seen[MB];
   float m[MB];
-  float4_t o[MB][D / 16 + 1];  // and the sums of the weights
+  float4_t o[MB][U / 16 + 1];  // and the sums of the weights
   const int wave_row0 = row0 + wave * MB * 16, wave_last = min(wave_row0 + MB * 16 - 1, last_row);
 #pragma unroll
   for (int u = 0; u < MB; u++) {
@@ -1098,7 +1101,7 @@ void cache_attention_rows(CacheView c, RowsView r, AttentionView a) {
     seen[u].init(keys, start + token);
     m[u] = -INFINITY;
 #pragma unroll
-    for (int d = 0; d <= D / 16; d++) o[u][d] = float4_t{0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d <= U / 16; d++) o[u][d] = float4_t{0.f, 0.f, 0.f, 0.f};
   }
   // What some of the wave's rows see of the ring's entries: nothing before some_from or from some_to on.
   const bool idle = wave_row0 > last_row;
@@ -1165,18 +1168,18 @@ void cache_attention_rows(CacheView c, RowsView r, AttentionView a) {
 
 #pragma unroll
   for (int u = 0; u < MB; u++) {
-    const float sum = X::row_sum(o[u][D / 16]), inv = 1.f / sum;
+    const float sum = X::row_sum(o[u][U / 16]), inv = 1.f / sum;
     const int row = wave_row0 + u * 16 + (lane & 15);
     if (row <= last_row && a.splits > 1) {
       const size_t at = (((size_t)b * c.kv_heads + head) * a.rows + row) * a.splits + split;
       if (g == 0) a.part_ml[at] = make_float2(m[u], sum);
 #pragma unroll
-      for (int d = 0; d < D / 16; d++)
+      for (int d = 0; d < U / 16; d++)
         if (d * 16 + g * 4 < c.dim) store_global(a.part_o + at * c.dim + d * 16 + g * 4, o[u][d]);
     } else if (row <= last_row) {
       const int token = row / a.group, h = head * a.group + row - token * a.group;
 #pragma unroll
-      for (int d = 0; d < D / 16; d++) {
+      for (int d = 0; d < U / 16; d++) {
         const float y[4] = {o[u][d][0] * inv, o[u][d][1] * inv, o[u][d][2] * inv, o[u][d][3] * inv};
         if (d * 16 + g * 4 < c.dim) store_out<A>(a, first + token, h, c.dim, d * 16 + g * 4, y);
       }

@@ -132,7 +132,10 @@ void launch_attention(const CacheView& c, const RowsView& r, const AttentionView
   auto go = [&](auto kernel, int threads) { hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, stream, c, r, a); };
   auto form = [&](auto D) {
     constexpr int d = decltype(D)::value;
-    if (p.many) return go(cache_attention_rows<A, C, d, d == 256 ? 1 : 2>, rows_threads(A, C, d));
+    if constexpr (d == 128) {  // head dimensions up to 96 in the same tiles, with a quarter of the products less
+      if (p.many && c.dim <= 96) return go(cache_attention_rows<A, C, d, 96, 2>, rows_threads(A, C, d));
+    }
+    if (p.many) return go(cache_attention_rows<A, C, d, d, d == 256 ? 1 : 2>, rows_threads(A, C, d));
     auto few = [&](auto NT) {
       constexpr bool nt = decltype(NT)::value;
       if constexpr (A == kTF32) {
