@@ -754,16 +754,31 @@ __global__ __launch_bounds__(64 * kWaves, 2 * 4 / kWaves) void cache_attention(C
 // so they are made by vector instructions, without LDS in the loop. A row of the cache is shared by L lanes, E
 // elements each; every group of L lanes takes keys of its own, with its own (m, l, O), and the groups and
 // waves are merged at the end. Each load's registers are loaded again as soon as they are used.
+// op over the lanes that share lane % L, in every lane: rotations within rows of 16, then swaps across rows.
+template <int L, typename Op>
+__device__ __forceinline__ float over_groups(float v, Op&& op) {
+  if constexpr (L <= 2) v = op(v, dpp_get<0x4E>(v));   // lane ^ 2
+  if constexpr (L <= 4) v = op(v, dpp_get<0x124>(v));  // row_ror:4: any two of lane % 4
+  if constexpr (L <= 8) v = op(v, dpp_get<0x128>(v));  // row_ror:8
+  float a, b;
+  if constexpr (L <= 16) {
+    swap_halves<false>(v, a, b);
+    v = op(a, b);
+  }
+  if constexpr (L <= 32) {
+    swap_halves<true>(v, a, b);
+    v = op(a, b);
+  }
+  return v;
+}
 template <int C, int D>
 constexpr int vector_loads() {  // loads of K (and of V) in flight per wave
   return C == kTInt4 ? 2 : 8;
 }
-constexpr int kVectorWaves = 8;
-template <int C, int D, int R, bool kNT>
-__global__ __launch_bounds__(64 * kVectorWaves) void cache_attention_vector(CacheView c, RowsView r, AttentionView a) {
+template <int C, int D, int R, int kWaves, bool kNT>
+__global__ __launch_bounds__(64 * kWaves) void cache_attention_vector(CacheView c, RowsView r, AttentionView a) {
   using Row = RowLoad<C, D>;
   constexpr int E = Row::E, L = Row::L, kGroups = 64 / L, NB = vector_loads<C, D>(), KT = NB * kGroups;
-  constexpr int kWaves = kVectorWaves;
   __shared__ __attribute__((aligned(16))) float merge[kWaves][R][D];
   __shared__ float ml[kWaves][2][R];
   const int split = blockIdx.x % a.splits, head = blockIdx.x / a.splits, b = blockIdx.y;
@@ -930,18 +945,13 @@ __global__ __launch_bounds__(64 * kVectorWaves) void cache_attention_vector(Cach
   // The wave's groups, then the waves.
 #pragma unroll
   for (int u = 0; u < R; u++) {
-    float top = m[u];
-#pragma unroll
-    for (int x = L; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+    const float top = over_groups<L>(m[u], [](float a, float b) { return fmaxf(a, b); });
     const float f = m[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[u] - top);
-    float sum = m[u] == -INFINITY ? l[u] : l[u] * f;
-#pragma unroll
-    for (int x = L; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
+    const auto add = [](float a, float b) { return a + b; };
+    const float sum = over_groups<L>(m[u] == -INFINITY ? l[u] : l[u] * f, add);
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      float y = o[u][e] * f;
-#pragma unroll
-      for (int x = L; x < 64; x <<= 1) y += __shfl_xor(y, x);
+      const float y = over_groups<L>(o[u][e] * f, add);
       if (sub == 0) merge[wave][u][p * E + e] = y;
     }
     if (lane == 0) {

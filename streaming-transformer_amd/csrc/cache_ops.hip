@@ -105,8 +105,14 @@ Plan plan_attention(const CacheView& c, const RowsView& r, int q_heads, int dtyp
   p.stream = 2 * pairs * keys * c.row_bytes > (int64_t)kStreamBytes;
   // Workgroups beside the splits, and as many as the chip holds at once.
   const int64_t base = pairs * p.tiles;
-  p.waves = p.vector || (p.blocks == 1 && padded < 256) ? 8 : 4;
-  const int64_t room = padded == 256 || p.waves == 8 ? 256 : 512;
+  // cache_attention_vector's workgroups end with a merge of all their lanes, which costs most over 4-bit rows (32
+  // groups of two lanes), so many short windows take two waves. us of eight / two, 8 heads of 64: 4-bit, 512 pairs
+  // 128 keys 12 / 9, 512 keys 17 / 15, 2048 keys 30 / 38; 1024 pairs 21 / 10, 31 / 16, 55 / 40; 4096 pairs 77 / 28,
+  // 112 / 51, 208 / 151. FP32, 512 pairs 7.7 / 8.1, 23 / 24; 1024 pairs 128 keys 16 / 14, 512 keys 42 / 44; 4096
+  // pairs 51 / 44, 161 / 166.
+  const bool two = stored == ST_TYPE_INT4 ? pairs >= (keys <= 1024 ? 512 : 1024) : pairs >= 1024 && keys <= 256;
+  p.waves = p.vector ? (two ? 2 : 8) : p.blocks == 1 && padded < 256 ? 8 : 4;
+  const int64_t room = padded == 256 || p.waves == 8 || p.vector ? 256 : 512;
   const int64_t share = p.waves * 32 * 2;  // fewest keys of a split: two tiles for each wave
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(room + base - 1) / base, keys / share, kMaxSplits}));
   return p;
@@ -139,10 +145,15 @@ void launch_attention(const CacheView& c, const RowsView& r, const AttentionView
     auto few = [&](auto NT) {
       constexpr bool nt = decltype(NT)::value;
       if constexpr (A == kTF32) {
-        if (p.vector == 1) return go(cache_attention_vector<C, d, 1, nt>, 64 * kVectorWaves);
-        if (p.vector == 2) return go(cache_attention_vector<C, d, 2, nt>, 64 * kVectorWaves);
+        auto rows = [&](auto R) {
+          constexpr int n = decltype(R)::value;
+          if (p.waves == 2) go(cache_attention_vector<C, d, n, 2, nt>, 128);
+          else go(cache_attention_vector<C, d, n, 8, nt>, 512);
+        };
+        if (p.vector == 1) return rows(std::integral_constant<int, 1>{});
+        if (p.vector == 2) return rows(std::integral_constant<int, 2>{});
         if constexpr (C != kTInt4) {
-          if (p.vector == 4) return go(cache_attention_vector<C, d, 4, nt>, 64 * kVectorWaves);
+          if (p.vector == 4) return rows(std::integral_constant<int, 4>{});
         }
       }
       if constexpr (d < 256) go(cache_attention<A, C, d, 1, 8, nt>, 512);
