@@ -71,6 +71,11 @@ __device__ __forceinline__ void store_cache(char* row, uint32_t* params, int e0,
 // per token (a pair per lane; the product with the position in 64 bits, which far positions need: the turn's
 // fraction then has 24 bits to spare for FP32) while the first heads are in flight. Pairs (i, i + half)
 // are exchanged through the wave's own LDS, 16 bytes at a time where half is a multiple of 8.
+//
+// Measured, 32 heads on 8 of 128, bfloat16: 16,384 tokens 89 us, 4.5 TB/s, bound by the bytes (a large copy reaches
+// 4.8); 256 tokens 6.3 us, one token 4.2: the launch and the chain of dependent loads (stream, position, heads).
+// Loading heads, frequencies and gains before the stream is looked up cost 0.8 us: loads return in order, so the
+// lookup then waits for them.
 template <int A, int C, int kTeam>
 __global__ __launch_bounds__(kAppendThreads) void cache_append(CacheView c, RowsView r, AppendView a) {
   constexpr int kTeams = kAppendThreads / kTeam, kAhead = 4;

@@ -123,7 +123,9 @@ size_t workspace_of(const CacheView& c, const RowsView& r, int q_heads, const Pl
   return (size_t)c.streams * q_heads * r.max_tokens * p.splits * (8 + (size_t)c.dim * 4);
 }
 
-// Tokens from which a wave takes one, else a workgroup.
+// Tokens from which a wave takes one, else a workgroup. us of a workgroup / a wave each, bfloat16, 32 heads on 8 of
+// 128: 256 tokens 7.0 / 12.5, 512 9.3 / 13.1, 1024 14.3 / 13.7, 2048 23.8 / 18.7, 4096 39.6 / 26.2; FP32, 16 on 16 of
+// 64: 256 tokens 6.1 / 8.5, 1024 11.3 / 10.0, 2048 18.5 / 14.4.
 constexpr int kWaveTokens = 1024;
 
 template <int A, int C>

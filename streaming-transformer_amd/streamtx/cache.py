@@ -4,8 +4,8 @@ Q/K/V projection and its output projection.
 ``KvCache`` holds keys and values with a sliding window and sinks, ``qk_norm_rope_append`` norms and
 rotates the heads of new tokens and appends their keys and values, ``window_attention`` attends over the
 cache. The calls launch on torch's current stream of the tensors' device, do not synchronize, and can be
-captured into a graph. Bad arguments raise ValueError, a failing library RuntimeError; there is no
-fallback. torch is imported by the first use, and has to be the HIP runtime that the library is
+captured into a graph. They have no gradients, and refuse tensors that ask for one where torch records
+them. Bad arguments raise ValueError, a failing library RuntimeError; there is no fallback. torch is imported by the first use, and has to be the HIP runtime that the library is
 loaded with: import torch before the first call into the library.
 """
 from __future__ import annotations
@@ -17,6 +17,7 @@ from . import runtime as _runtime
 
 __all__ = ['KvCache', 'qk_norm_rope_append', 'window_attention']
 
+_MOST = 1 << 30  # rows, slots: far below what 32-bit fields hold
 GROUP = 32  # values that share a (scale, minimum) pair in a 4-bit cache
 _F32, _F16, _BF16, _INT4 = range(4)
 
@@ -76,9 +77,15 @@ def _need(ok, message):
         raise ValueError(message)
 
 
+def _no_gradients(*tensors):
+    if _torch.is_grad_enabled():
+        _need(not any(t is not None and t.requires_grad for t in tensors),
+              'the cache operators have no gradients: call them under torch.no_grad()')
+
+
 def _sig(t):
     """All that the checks ask of a tensor argument but its address."""
-    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device(), t.requires_grad)
 
 
 class KvCache:
@@ -94,7 +101,8 @@ class KvCache:
 
     `positions` (int64, [streams], on the device) counts the tokens that each stream has; -1 leaves a stream
     out of a call. The operators read it; :meth:`advance` adds a call's tokens once every layer has them (the
-    layers of a model may share one tensor of positions)."""
+    layers of a model may share one tensor of positions). A cache keeps its tensors: write into them, none can
+    be replaced."""
 
     def __init__(self, streams, kv_heads, head_dim, window, sinks=0, max_tokens=1, dtype=None, device=None, positions=None):
         torch, _ = _load()
@@ -125,6 +133,7 @@ class KvCache:
 
     def _adopt(self, keys, values, positions, window, sinks, key_params, value_params):
         torch, _ = _load()
+        _no_gradients(keys, values, key_params, value_params)
         int4 = key_params is not None or value_params is not None
         _need(keys.dim() == 4 and keys.shape == values.shape and keys.dtype == values.dtype,
               'keys and values must be tensors of one shape [streams, kv_heads, slots, row] and type')
@@ -144,6 +153,7 @@ class KvCache:
         window, sinks = int(window), int(sinks)
         ring = slots - sinks
         _need(window >= 1 and sinks >= 0 and ring >= window, 'a cache needs sinks + window slots at least')
+        _need(slots <= _MOST, 'a cache has at most 2^30 slots')
         strides = self._row_strides(keys, row)
         _need(strides is not None and self._row_strides(values, row) == strides,
               'keys and values must have the same strides, in whole rows')
@@ -164,6 +174,14 @@ class KvCache:
                               value_params.data_ptr() if int4 else None, positions.data_ptr())
         self._address = ctypes.addressof(self._struct)
         self._plans = {}  # checked argument structs by the arguments' shapes, strides and types
+        self._fixed = True
+
+    def __setattr__(self, name, value):
+        # The struct holds the tensors' addresses: one put in a tensor's place would never be read. (x += y on an
+        # attribute assigns the tensor that is there, which is fine.)
+        if getattr(self, '_fixed', False) and value is not getattr(self, name, None):
+            raise AttributeError(f'{name} of a cache is fixed: write into its tensors')
+        object.__setattr__(self, name, value)
 
     @staticmethod
     def _row_strides(t, row):
@@ -213,11 +231,14 @@ class KvCache:
             _need(max_tokens is None or max_tokens == n, 'max_tokens goes with offsets')
             if n == 0:
                 return 0, None
+            _need(self.streams * n <= _MOST, 'a call has at most 2^30 tokens')
             return self.streams * n, _Rows(self.streams * n, n, None)
         _need(q.dim() == 3, 'with offsets q is [tokens, heads, head_dim]')
         _need(offsets.dtype == torch.int32 and offsets.shape == (self.streams + 1,) and offsets.is_contiguous()
               and offsets.device == self.device, 'offsets must be int32 [streams + 1] on the cache\'s device')
         _need(max_tokens is not None, 'offsets need max_tokens, the most tokens of one stream')
+        _need(q.shape[0] <= _MOST and 1 <= max_tokens <= self.max_tokens,
+              f'a call has at most 2^30 tokens, and this cache takes 1 to {self.max_tokens} of one stream')
         return q.shape[0], _Rows(q.shape[0], max_tokens, offsets.data_ptr())
 
     def _heads(self, t, like, heads, name, dtype):
@@ -232,7 +253,6 @@ class KvCache:
             _need(s[0] == s[1] * shape[1], f'the tokens of {name} must be evenly spaced over the streams')
             return s[1], s[2]
         return (s[0] if len(shape) == 4 and shape[0] > 1 else s[-3]), s[-2]
-
 
     def _plan(self, key, make):
         """The checked structs of a call; the same shapes, strides and types are checked once."""
@@ -260,10 +280,12 @@ def _launch(device, call, *args):
 
 def _plan_append(cache, q, k, v, q_gain, k_gain, inv_freq, rope, rope_dims, pairs, offsets, max_tokens, out):
     torch = _torch
+    _no_gradients(q, k, v, q_gain, k_gain, inv_freq, rope, out)
     tokens, rows = cache._rows(q, offsets, max_tokens)
     dtype = q.dtype
     _need(dtype in _types, 'q must be float32, float16 or bfloat16')
     heads = q.shape[-2]
+    _need(heads <= 65535, 'at most 65535 query heads')
     args = _Append()
     args.dtype, args.q_heads = _types[dtype], heads
     args.q_strides = cache._heads(q, q, heads, 'q', dtype)
@@ -310,7 +332,7 @@ def qk_norm_rope_append(cache, q, k, v, *, q_gain=None, k_gain=None, epsilon=1e-
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     key = (_sig(q), _sig(k), _sig(v), _sig(q_gain), _sig(k_gain), _sig(inv_freq), _sig(rope), rope_dims, pairs, _sig(offsets),
-           max_tokens, _sig(out))
+           max_tokens, _sig(out), torch.is_grad_enabled())
     tokens, rows, args = cache._plan(key, lambda: _plan_append(cache, q, k, v, q_gain, k_gain, inv_freq, rope, rope_dims, pairs,
                                                                offsets, max_tokens, out))
     if not tokens:
@@ -333,10 +355,12 @@ def qk_norm_rope_append(cache, q, k, v, *, q_gain=None, k_gain=None, epsilon=1e-
 
 
 def _plan_attention(cache, q, offsets, max_tokens, out):
+    _no_gradients(q, out)
     tokens, rows = cache._rows(q, offsets, max_tokens)
     dtype = q.dtype
     _need(dtype in _types, 'q must be float32, float16 or bfloat16')
     heads = q.shape[-2]
+    _need(heads <= 65535, 'at most 65535 query heads')
     args = _Attention()
     args.dtype, args.q_heads = _types[dtype], heads
     args.q_strides = cache._heads(q, q, heads, 'q', dtype)
@@ -359,7 +383,7 @@ def window_attention(cache, q, *, scale=None, offsets=None, max_tokens=None, out
     _need(isinstance(cache, KvCache), 'cache must be a KvCache')
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    key = (_sig(q), _sig(offsets), max_tokens, _sig(out))
+    key = (_sig(q), _sig(offsets), max_tokens, _sig(out), torch.is_grad_enabled())
     tokens, rows, args = cache._plan(key, lambda: _plan_attention(cache, q, offsets, max_tokens, out))
     if not tokens:
         return out

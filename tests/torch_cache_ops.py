@@ -168,11 +168,53 @@ def refusals():
     torch.cuda.synchronize()
 
 
+def fixed():
+    """A cache's tensors cannot be replaced (the library has their addresses), rows beyond 32 bits and tensors
+    that ask for gradients are refused; writing in place, and the same calls without gradients, go through."""
+    c = KvCache(2, 2, 64, 8, 1, 3, torch.float16, DEV)
+    q, k = (torch.ones(2, 1, h, 64, dtype=torch.float16, device=DEV) for h in (4, 2))
+    at = torch.tensor([0, 1, 2], dtype=torch.int32, device=DEV)
+    for name in ('positions', 'keys', 'values', 'window', 'sinks'):
+        try:
+            setattr(c, name, getattr(c, name) + 1)
+        except AttributeError as e:
+            assert 'fixed' in str(e), str(e)
+        else:
+            raise AssertionError(name)
+    c.positions += 1
+    assert c.positions.tolist() == [1, 1]
+    wide = torch.empty(1, 1, 4, 64, dtype=torch.float16, device=DEV)
+    grad = q.clone().requires_grad_()
+    bad = [
+        (lambda: window_attention(c, wide[0].expand(2**32 + 2, 4, 64), out=wide[0].expand(2**32 + 2, 4, 64), offsets=at,
+                                  max_tokens=1), '2^30'),
+        (lambda: window_attention(c, wide.expand(2, 2**31 + 1, 4, 64), out=wide.expand(2, 2**31 + 1, 4, 64)), '2^30'),
+        (lambda: window_attention(c, q[:, 0], offsets=at, max_tokens=2**32 + 1), 'takes 1 to 3'),
+        (lambda: window_attention(c, q[:, 0], offsets=at, max_tokens=0), 'takes 1 to 3'),
+        (lambda: window_attention(c, grad), 'no_grad'),
+        (lambda: qk_norm_rope_append(c, q, k, k, q_gain=torch.ones(64, device=DEV, requires_grad=True)), 'no_grad'),
+        (lambda: qk_norm_rope_append(c, q, k.clone().requires_grad_(), k), 'no_grad'),
+    ]
+    for i, (call, match) in enumerate(bad):
+        try:
+            call()
+        except ValueError as e:
+            assert match in str(e), (i, match, str(e))
+        else:
+            raise AssertionError((i, match))
+    with torch.no_grad():
+        qk_norm_rope_append(c, grad, k, k)
+        out = window_attention(c, grad)
+    # Slot 0 holds zeros (nothing appended it), slot 1 ones: q . k = 0 and 64, over sqrt(64).
+    want = math.exp(8) / (1 + math.exp(8))
+    assert not out.requires_grad and (out.double() - want).abs().max().item() <= 4 * STEP[torch.float16] + 2.0**-18
+
+
 if __name__ == '__main__':
     for dtype, stored in ((torch.float32, torch.float32), (torch.bfloat16, 'int4'), (torch.float32, torch.float16)):
         print('generation', dtype, stored, flush=True)
         generation(dtype, stored, True)
-    for check in (other_stream, captured, refusals):
+    for check in (other_stream, captured, refusals, fixed):
         print(check.__name__, flush=True)
         check()
     torch.cuda.synchronize()
