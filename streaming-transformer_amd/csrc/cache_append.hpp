@@ -65,7 +65,8 @@ __device__ __forceinline__ void store_cache(char* row, uint32_t* params, int e0,
 }
 
 // A team of kTeam threads per token: the workgroup for few tokens, a wave for many (four tokens per workgroup,
-// and no barrier). A head is shared by G = 2^lane_shift lanes, eight elements (16 bytes, 32 of FP32) each, and
+// and no barrier), a quarter of a wave where those have few heads (then the teams of a wave return apart, and
+// nothing crosses them). A head is shared by G = 2^lane_shift lanes, eight elements (16 bytes, 32 of FP32) each, and
 // the team's kTeam / G groups walk the token's query, key and value heads, four of a group in flight. A lane's
 // elements are the same of every head, so its gains and angles stay in registers. The angles are computed once
 // per token (a pair per lane; the product with the position in 64 bits, which far positions need: the turn's
@@ -85,14 +86,19 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append(CacheView c, Rows
   const int wave = wave_id(), lane = lane_id();
   const int thread = threadIdx.x % kTeam;  // of the team
   float2* const turn = turns[threadIdx.x / kTeam];
-  const int row = blockIdx.x * kTeams + (kTeam == 64 ? wave : 0);
+  const int row = blockIdx.x * kTeams + (kTeam == 64 ? wave : threadIdx.x / kTeam);
   if (kTeams > 1 && row >= r.tokens) return;
   int b, index;
   if (r.offsets) {
     int before = 0;  // streams that end at or before this row
-    for (int i = lane; i < ((c.streams + 63) & ~63); i += 64)
-      before += __builtin_popcountll(__ballot(i < c.streams && r.offsets[min(i, c.streams - 1) + 1] <= row));
-    before = __builtin_amdgcn_readfirstlane(before);
+    if constexpr (kTeam < 64) {
+      for (int i = thread; i < c.streams; i += kTeam) before += r.offsets[i + 1] <= row;
+      before = (int)group_sum((float)before, kTeam);
+    } else {
+      for (int i = lane; i < ((c.streams + 63) & ~63); i += 64)
+        before += __builtin_popcountll(__ballot(i < c.streams && r.offsets[min(i, c.streams - 1) + 1] <= row));
+      before = __builtin_amdgcn_readfirstlane(before);
+    }
     if (before >= c.streams) return;
     int first, n;
     stream_rows(r, before, first, n);
@@ -142,7 +148,7 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append(CacheView c, Rows
     gq[i] = a.q_gain ? a.q_gain[at + i] : 1.f;
     gk[i] = a.k_gain ? a.k_gain[at + i] : 1.f;
   }
-  if constexpr (kTeam == 64) wave_sync();
+  if constexpr (kTeam <= 64) wave_sync();
   else __syncthreads();
   // Element i of the lane is rotated with its partner y: x cos - y sin (first of its pair) or x cos + y sin.
   // Elements that do not rotate: cos 1, and no partner.

@@ -59,17 +59,18 @@ void check_heads(const st_kv_cache* cache, const st_new_rows* rows, int q_heads)
 // Head dimension of the kernels: the smallest that holds it.
 int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
-// cache_attention_rows is taken where it has kManyWaves waves, which is half of what the chip holds, by itself or
+// cache_attention_rows is taken where it has kManyWaves waves, three eighths of what the chip holds, by itself or
 // split along the keys into shares of kManyKeys or more. us of cache_attention (split) / cache_attention_rows, 32
-// heads on 8, head dimension 128, bfloat16: 128 tokens and a window of 1024, one stream 25 / 34 (128 waves), four
-// 34 / 35 (512), 16 118 / 54 (2048); window 8192, one stream 57 / 45 (128 waves x 8 splits), four 168 / 101 (512 x
-// 4), 16 621 / 306; one stream of 512 tokens 158 / 97. Over 4-bit rows, eight streams, window 2048: 32 tokens 41 /
-// 54 (512 waves x 2), 128 tokens 100 / 83 (1024).
+// heads on 8, head dimension 128, bfloat16: 128 tokens and a window of 1024, one stream 25 / 35 (128 waves), four
+// 35 / 36 (512), 16 123 / 57 (2048); window 8192, one stream 57 / 46 (128 waves x 8 splits), four 159 / 105 (512 x
+// 4), 16 613 / 306; one stream of 512 tokens 155 / 100. 12 on 3 of 64, FP16, window 512: 1186 tokens 17 / 18 (456),
+// 2400 32 / 20 (912); window 22 10 / 9, 18 / 9. Over 4-bit rows, eight streams, window 2048: 32 tokens 41 / 54 (512
+// waves x 2), 128 tokens 100 / 83 (1024).
 // Rows per (stream, cache head) above which: a wave of theirs has 32, so fewer leave waves idle, and FP32 products
 // or converted rows cost those that work more. 64 streams, window 1024, 32 rows 52 / 55, 36 rows 65 / 52; 4-bit 96
 // rows 92 / 97, 128 rows 115 / 95; FP32 (32 streams, window 512) 64 rows 71 / 103, 128 rows 130 / 114.
 constexpr int kManyRows = 32, kManyRowsSlow = 96;
-constexpr int kManyWaves = 1024, kManySplit = 2048, kManyKeys = 1024;
+constexpr int kManyWaves = 768, kManySplit = 2048, kManyKeys = 1024;
 constexpr size_t kStreamBytes = (size_t)256 << 20;  // the Infinity Cache
 
 struct Plan {
@@ -85,11 +86,15 @@ Plan plan_attention(const CacheView& c, const RowsView& r, int q_heads, int dtyp
   Plan p{};
   const int rows = r.max_tokens * (q_heads / c.kv_heads), padded = padded_dim(c.dim);
   const int64_t pairs = (int64_t)c.streams * c.kv_heads;
-  const int64_t keys = (int64_t)c.sinks + std::min<int64_t>(c.ring, (int64_t)c.window + r.max_tokens - 1);
+  // Most keys of a tile of rows: its tokens' windows together.
+  const auto keys_of = [&](int tile) {
+    return (int64_t)c.sinks + c.window + std::min(r.max_tokens, (tile - 1) / (q_heads / c.kv_heads) + 2) - 1;
+  };
   if (rows > (dtype != ST_TYPE_F32 && dtype == stored ? kManyRows : kManyRowsSlow)) {
     const int waves = rows_waves(dtype, stored, padded), blocks = padded == 256 ? 1 : 2, tile = 16 * blocks * waves;
     p.tiles = (rows + tile - 1) / tile;
-    const int64_t base = pairs * p.tiles, splits = std::min<int64_t>({kManySplit / (base * waves), keys / kManyKeys, kMaxSplits});
+    const int64_t base = pairs * p.tiles;
+    const int64_t splits = std::min<int64_t>({kManySplit / (base * waves), keys_of(tile) / kManyKeys, kMaxSplits});
     if (base * waves >= kManyWaves || (splits >= 4 && base * waves * splits >= kManyWaves)) {
       p.many = true;
       p.blocks = blocks;
@@ -102,8 +107,9 @@ Plan plan_attention(const CacheView& c, const RowsView& r, int q_heads, int dtyp
   const int group = q_heads / c.kv_heads;
   // Four query heads over 4-bit rows, 32 elements of each to a lane, do not fit into registers.
   if (dtype == ST_TYPE_F32 && r.max_tokens == 1 && group <= (stored == ST_TYPE_INT4 ? 2 : 4)) p.vector = group == 3 ? 4 : group;
+  const int64_t keys = keys_of(16 * p.blocks);
   p.stream = 2 * pairs * keys * c.row_bytes > (int64_t)kStreamBytes;
-  // Workgroups beside the splits, and as many as the chip holds at once.
+  // Workgroups beside the splits.
   const int64_t base = pairs * p.tiles;
   // cache_attention_vector's workgroups end with a merge of all their lanes, which costs most over 4-bit rows (32
   // groups of two lanes), so many short windows take two waves. us of eight / two, 8 heads of 64: 4-bit, 512 pairs
@@ -114,7 +120,10 @@ Plan plan_attention(const CacheView& c, const RowsView& r, int q_heads, int dtyp
   p.waves = p.vector ? (two ? 2 : 8) : p.blocks == 1 && padded < 256 ? 8 : 4;
   const int64_t room = padded == 256 || p.waves == 8 || p.vector ? 256 : 512;
   const int64_t share = p.waves * 32 * 2;  // fewest keys of a split: two tiles for each wave
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(room + base - 1) / base, keys / share, kMaxSplits}));
+  // As many as the chip holds at once and no more, since a second round costs more than idle CUs: us of 3 / 4 splits,
+  // 37 streams, two heads (222 / 296 workgroups for 256 CUs), window 3438 28 / 35, head dimension 256 52 / 72, 4-bit
+  // (8192) 32 / 45; 1 / 2 splits, 75 streams, window 2048 29 / 39, 8192 118 / 132.
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({room / base, keys / share, kMaxSplits}));
   return p;
 }
 
@@ -127,10 +136,18 @@ size_t workspace_of(const CacheView& c, const RowsView& r, int q_heads, const Pl
 // 128: 256 tokens 7.0 / 12.5, 512 9.3 / 13.1, 1024 14.3 / 13.7, 2048 23.8 / 18.7, 4096 39.6 / 26.2; FP32, 16 on 16 of
 // 64: 256 tokens 6.1 / 8.5, 1024 11.3 / 10.0, 2048 18.5 / 14.4.
 constexpr int kWaveTokens = 1024;
+// Few heads (queries', keys' and values' at 8 elements a lane: kFewLanes lanes, twice that from kManyTokens on) leave
+// most of a wave idle: 16 lanes a token then. us of 16 / 64 lanes, bfloat16: 32,768 tokens, two heads on one of 64 (32
+// lanes) 18 / 43, four on two of 128 (128) 38 / 69, eight on two (192) 46 / 72, 32 on 8 (768) 179 / 166; 4096 tokens
+// 6.6 / 8.8, 12 / 13, 15 / 14, 39 / 26.
+constexpr int kFewLanes = 128, kFewTokens = 4096, kManyTokens = 16384;
 
 template <int A, int C>
 void launch_append(const CacheView& c, const RowsView& r, const AppendView& a, hipStream_t stream) {
-  if (r.tokens < kWaveTokens) hipLaunchKernelGGL((cache_append<A, C, 256>), dim3(r.tokens), dim3(kAppendThreads), 0, stream, c, r, a);
+  const int lanes = (a.q_heads + 2 * c.kv_heads) << a.lane_shift;
+  if (r.tokens >= kFewTokens && a.lane_shift <= 4 && lanes <= (r.tokens >= kManyTokens ? 2 * kFewLanes : kFewLanes))
+    hipLaunchKernelGGL((cache_append<A, C, 16>), dim3((r.tokens + 15) / 16), dim3(kAppendThreads), 0, stream, c, r, a);
+  else if (r.tokens < kWaveTokens) hipLaunchKernelGGL((cache_append<A, C, 256>), dim3(r.tokens), dim3(kAppendThreads), 0, stream, c, r, a);
   else hipLaunchKernelGGL((cache_append<A, C, 64>), dim3((r.tokens + 3) / 4), dim3(kAppendThreads), 0, stream, c, r, a);
 }
 

@@ -51,16 +51,17 @@ APPEND = [  # dim, q heads, kv heads, rotated, halves, norm, pad
 ]
 
 
-@pytest.mark.parametrize('types', PAIRS, ids=pair_id)
-@pytest.mark.parametrize('shape', APPEND, ids=str)
-def test_append(types, shape):
+def run_append(types, shape, starts, n, counts=None):
     dtype, stored = types
     dim, heads, kv, rope_dims, halves, norm, pad = shape
     rng = np.random.default_rng(dim + heads)
-    n, window, sinks = 3, 9, 2
-    starts = [0, 5, 1000003, 1]
-    cache = Cache(4, kv, dim, window, sinks, stored, max_tokens=n, positions=starts)
-    rows, firsts, total = rows_struct(cache, n=n)
+    window, sinks = 9, 2
+    cache = Cache(len(starts), kv, dim, window, sinks, stored, max_tokens=n, positions=starts)
+    offsets = None
+    if counts is not None:
+        offsets = Device(np.concatenate(([0], np.cumsum(counts))).astype(np.int32))
+    rows, firsts, total = rows_struct(cache, counts, n, offsets)
+    counts = [n] * len(starts) if counts is None else counts
     q, k, v = (Heads(rng.standard_normal((total, h, dim)) * 2, dtype, pad) for h in (heads, kv, kv))
     out = Heads(np.zeros((total, heads, dim)), dtype, pad)
     gq, gk = (1 + 0.2 * rng.standard_normal(dim).astype(np.float32) for _ in range(2)) if norm else (None, None)
@@ -68,37 +69,70 @@ def test_append(types, shape):
     dev = [Device(g) if g is not None else None for g in (gq, gk)]
     inv = Device(freq) if rope_dims else None
     append(cache, rows, q, k, v, out, *dev, inv_freq=inv, rope_dims=rope_dims, halves=halves)
-    angles = angles_of(starts, firsts, [n] * 4, total, freq)
+    angles = angles_of(starts, firsts, counts, total, freq)
     got, clean = out.get()
     assert clean
     want, size = turned(q.float(), gq, 1e-6, angles, rope_dims, halves)
+    for start, first, m in zip(starts, firsts, counts):
+        if start < 0:
+            want[first:first + m] = size[first:first + m] = 0
     assert (np.abs(got - want) <= norm_bound(want, size, dtype)).all()
 
     kw, size = turned(k.float(), gk, 1e-6, angles, rope_dims, halves)
     stored_rows = cache.values()
     untouched = np.ones(cache.dims, bool)
-    for b in range(4):
-        at = cache.slot(starts[b] + np.arange(n))
+    raw = cache.raw()
+    for b in range(len(starts)):
+        if starts[b] < 0 or not counts[b]:
+            continue
+        at = cache.slot(starts[b] + np.arange(counts[b]))
         untouched[b][:, at] = False
-        part = slice(firsts[b], firsts[b] + n)
+        part = slice(firsts[b], firsts[b] + counts[b])
         keys, values = (x[b][:, at].transpose(1, 0, 2) for x in stored_rows)
         if stored == INT4:
             # Keys: the nearest code of a range that is itself rounded to FP16.
             codes, params = (x[b][:, at].transpose(1, 0, 2) if x.ndim == 4 else x[b][:, at].transpose(1, 0, 2, 3)
-                             for x in cache.raw()[0:3:2])
+                             for x in raw[0:3:2])
             p = params.astype(np.float64)
             step = np.repeat(p[..., 0], 32, -1)
             ends = np.repeat(np.abs(p[..., 1]) + 15 * p[..., 0], 32, -1)
             assert (np.abs(keys - kw[part]) <= step / 2 + ends * 2 * STEP[F16] + norm_bound(kw, size, F32)[part]).all()
             # Values come as they are: the format's own arithmetic, bit for bit.
             want_codes, want_params = quantise(v.float()[part].astype(np.float32))
-            assert (unpack(cache.raw()[1][b][:, at].transpose(1, 0, 2)) == want_codes).all()
-            assert (cache.raw()[3][b][:, at].transpose(1, 0, 2, 3) == want_params).all()
+            assert (unpack(raw[1][b][:, at].transpose(1, 0, 2)) == want_codes).all()
+            assert (raw[3][b][:, at].transpose(1, 0, 2, 3) == want_params).all()
         else:
             assert (np.abs(keys - kw[part]) <= norm_bound(kw, size, stored)[part]).all()
             assert (values == decode(encode(v.float()[part], stored), stored)).all()
-    for x in cache.raw():
+    for x in raw:
         assert (x[untouched] == 0).all()
+
+
+@pytest.mark.parametrize('types', PAIRS, ids=pair_id)
+@pytest.mark.parametrize('shape', APPEND, ids=str)
+def test_append(types, shape):
+    run_append(types, shape, [0, 5, 1000003, 1], 3)
+
+
+@pytest.mark.parametrize('types', PAIRS, ids=pair_id)
+@pytest.mark.parametrize('shape', [
+    (96, 3, 3, 48, 1, True, 0),   # 1300 tokens
+    (64, 2, 1, 64, 1, True, 0),   # 4225 tokens of few heads
+    (32, 3, 1, 16, 0, True, 32),
+    (128, 2, 1, 90, 1, True, 0),
+], ids=str)
+def test_append_many_tokens(types, shape):
+    """Unequal numbers of tokens, none among them, and a stream that is left out."""
+    n = 400 if shape[0] == 96 else 1300
+    run_append(types, shape, [0, 7, 12345, -5, 1], n, [n, 0, 3 * n // 4, n, n // 2])
+
+
+def test_append_a_token_of_each_of_many_streams():
+    run_append((BF16, INT4), (64, 1, 1, 64, 1, True, 0), [b * 7 if b % 5 else -1 for b in range(5003)], 1)
+
+
+def test_append_a_long_prompt():
+    run_append((BF16, BF16), (128, 8, 2, 128, 1, True, 0), [3], 16500)
 
 
 def test_append_in_place_and_from_a_table():
