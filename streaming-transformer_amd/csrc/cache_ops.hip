@@ -117,7 +117,11 @@ Plan plan_attention(const CacheView& c, const RowsView& r, int q_heads, int dtyp
   // 112 / 51, 208 / 151. FP32, 512 pairs 7.7 / 8.1, 23 / 24; 1024 pairs 128 keys 16 / 14, 512 keys 42 / 44; 4096
   // pairs 51 / 44, 161 / 166.
   const bool two = stored == ST_TYPE_INT4 ? pairs >= (keys <= 1024 ? 512 : 1024) : pairs >= 1024 && keys <= 256;
-  p.waves = p.vector ? (two ? 2 : 8) : p.blocks == 1 && padded < 256 ? 8 : 4;
+  // cache_attention: eight waves a CU, in one workgroup, or in two where there are more than one round of those. us of
+  // eight / four, bfloat16, 32 heads on 8 of 128: 32 streams (256 workgroups), window 64 8.0 / 7.6, 512 15 / 19, 1024
+  // 25 / 29; 64 streams, 64 13 / 8.0, 256 22 / 18, 1024 49 / 47, 4096 168 / 167; 256 streams, 128 60 / 39, 1024 179 /
+  // 166; 4 bits 58 / 34, 105 / 85.
+  p.waves = p.vector ? (two ? 2 : 8) : p.blocks == 1 && padded < 256 && base <= 256 ? 8 : 4;
   const int64_t room = padded == 256 || p.waves == 8 || p.vector ? 256 : 512;
   const int64_t share = p.waves * 32 * 2;  // fewest keys of a split: two tiles for each wave
   // As many as the chip holds at once and no more, since a second round costs more than idle CUs: us of 3 / 4 splits,
@@ -175,8 +179,10 @@ void launch_attention(const CacheView& c, const RowsView& r, const AttentionView
           if (p.vector == 4) return rows(std::integral_constant<int, 4>{});
         }
       }
-      if constexpr (d < 256) go(cache_attention<A, C, d, 1, 8, nt>, 512);
-      else go(cache_attention<A, C, d, 1, 4, nt>, 256);
+      if constexpr (d < 256) {
+        if (p.waves == 8) return go(cache_attention<A, C, d, 1, 8, nt>, 512);
+      }
+      go(cache_attention<A, C, d, 1, 4, nt>, 256);
     };
     if constexpr (d < 256) {
       if (p.blocks == 2) return go(cache_attention<A, C, d, 2, 4, false>, 256);
