@@ -556,7 +556,7 @@ __device__ __forceinline__ void store_out(const AttentionView& a, int row, int h
 //
 // Measured, bfloat16, 32 heads on 8 of 128, single tokens: 64 streams and a window of 4096 166 us (6.45 TB/s); one
 // stream, FP16, a window of 131,072 89 us (6.0 TB/s, with the merge of its splits); 64 streams over 8191 rows of 4
-// bits 137 us (4.9 TB/s): those are bound by the instructions that unpack a row, 1.7 per element.
+// bits 130 us (5.1 TB/s): those are bound by the instructions that unpack a row, 1.7 per element.
 //
 // A masked key's weight is an exact zero, but zero times a value that is not finite is NaN: tiles that are
 // not seen whole look for such values as they are staged, and where there is one they are added apart, for
@@ -1001,9 +1001,9 @@ __global__ __launch_bounds__(64 * kWaves) void cache_attention_vector(CacheView 
 // Measured, 32 heads on 8 of 128: 8192 tokens, bfloat16, a window of 2048 264 us (910 TF/s of the 1107 that a large
 // matrix product reaches): the exponentials and packing between the two products share the issue slots with them,
 // and two workgroups per CU overlap most of it. Tiles of 32 keys 316 us, of 128 517; waves of 16 rows 422; eight
-// waves 288. Four streams of 1024 FP16 tokens over 4-bit rows, window 4096: 470 us; K in two terms is half as many
+// waves 288. Four streams of 1024 FP16 tokens over 4-bit rows, window 4096: 465 us; K in two terms is half as many
 // products again. Ragged pieces of up to 333 tokens (19 streams, head dimension 80) 51 us: about 2 us for each tile
-// of a workgroup's chain of 15 and 15 us before and after it, with half of the waves the chip holds.
+// of a workgroup's chain of 13 and some 20 us before and after it, with fewer workgroups than the chip holds.
 template <int M, int D>
 constexpr int rows_tile() {
   return M == kTF32 ? 4096 / D : D == 256 ? 32 : 64;

@@ -71,7 +71,9 @@ int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 // rows 92 / 97, 128 rows 115 / 95; FP32 (32 streams, window 512) 64 rows 71 / 103, 128 rows 130 / 114.
 constexpr int kManyRows = 32, kManyRowsSlow = 96;
 constexpr int kManyWaves = 768, kManySplit = 2048, kManyKeys = 1024;
-constexpr size_t kStreamBytes = (size_t)256 << 20;  // the Infinity Cache
+// The Infinity Cache: a larger cache is read with non-temporal loads where each row is read once. 1.07 GB of bfloat16 by
+// 64 streams' single tokens 186 us without, 166 with; 0.6 GB of 4-bit rows 165 / 155.
+constexpr size_t kStreamBytes = (size_t)256 << 20;
 
 struct Plan {
   bool many;   // cache_attention_rows
