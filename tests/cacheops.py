@@ -310,7 +310,7 @@ def attention_bound(out, mass, size, keys, cache, dtype):
     two sums of `keys` such terms, numerator and denominator off alike: twice. 16-bit products round each
     weight once (half a step; FP16 also up to 2^-25 of the largest weight below its smallest normal number)
     and the output once. 4-bit rows that go to 16-bit products are rounded to FP16: keys within the
-    logits, values within the sum."""
+    logits, values within the sum. (Where a kernel takes weights or keys in two terms it is closer than that.)"""
     u = 2.0**-24
     top = max(np.abs(cache.values()[1]).max(), 1e-30)
     logit = (cache.dim + 6) * u * size[..., None]
