@@ -38,6 +38,7 @@ Batch::Batch(const st_config& config, bool mixed, const st_tensor* tensors, size
   if (options.kv_dtype < ST_KV_AS_MODEL || options.kv_dtype > ST_TYPE_INT4) throw Error(ST_ERR_INVALID, "Unknown K/V storage");
   if (options.sinks < 0 || options.sinks > 4096) throw Error(ST_ERR_INVALID, "Sinks must be between 0 and 4096");
   if (options.head_norm != 0 && options.head_norm != 1) throw Error(ST_ERR_INVALID, "head_norm must be 0 or 1");
+  if (options.head_norm && !(c_.epsilon >= 1e-37f)) throw Error(ST_ERR_INVALID, "Head norms need an epsilon of at least 1e-37");
   kv_type_ = options.kv_dtype == ST_KV_AS_MODEL ? ST_TYPE_F32 : options.kv_dtype;
   cached_ = options.sinks || options.head_norm || kv_type_ != ST_TYPE_F32 || (mixed && options.kv_dtype != ST_KV_AS_MODEL);
   slots_ = c_.window + options.sinks;

@@ -40,6 +40,11 @@ def test_combinations_refused():
             BatchRuntime((CONFIG, w, False), 2, options=BatchOptions(), **more)
 
 
+def test_head_norms_refuse_an_epsilon_below_normal_numbers():
+    w = dict(synthetic_checkpoint(CONFIG, seed=0), **{f'layers.0.{n}': np.ones(32, np.float32) for n in ('q_norm', 'k_norm')})
+    refused('epsilon', ModelConfig(1, 64, 2, 128, 16, 32, epsilon=1e-38), tensors=w, head_norm=1)
+
+
 def test_default_options():
     o = _BatchOptions(9, 9, 9, 9)
     library().st_batch_options_default(ctypes.byref(o))
